@@ -658,6 +658,115 @@ int mv_prefill_plan(const int64_t* seq_rows, const int64_t* cached_len, const in
                     int32_t num_kv_heads, int64_t* seqs, int32_t* work_items,
                     int32_t work_capacity, int32_t* status, void* stream);
 
+/* ------------------------------------------------- the 8-bit KV cache --
+ *
+ * Pools of e4m3 codes (one byte, OCP e4m3fn) in the layout above and, per
+ * layer, kv_scales float[num_blocks][num_kv_heads][2]: one scale for K and one
+ * for V of each (block, kv head). An entry stands for code * scale. Scales are
+ * powers of two, 2^-110 or more, and 0 for a block never written: a pool starts
+ * with its scales zeroed. Rows are fp16 or bf16; block_size is a power of two
+ * from 16 to 256, head_dim 64 or 128. (The reference's cache holds the model's
+ * type only.)
+ */
+
+/* Status words of mv_fp8_write_plan (int32[MV_FP8_PLAN_WORDS], device). */
+#define MV_FP8_PLAN_OUT_OF_RANGE 0 /* # slots < -1 or >= num_blocks * block_size */
+#define MV_FP8_PLAN_REPEATED 1     /* # tokens whose slot another token has too */
+#define MV_FP8_PLAN_POSITIONS 2    /* # positions outside [0, max_positions) */
+#define MV_FP8_PLAN_ITEMS 3        /* touched blocks */
+#define MV_FP8_PLAN_WORDS 4
+
+/*
+ * The plan of a step's appends, shared by its layers: the step's tokens by
+ * block. slot_mapping int64[num_tokens], -1 skips a token; positions
+ * int64[num_tokens] or NULL (not checked). Writes items int32[num_tokens]
+ * (the touched blocks, status[MV_FP8_PLAN_ITEMS] of them, in no fixed order)
+ * and table int32[num_tokens * block_size] (per item and place the token, or
+ * -1; of a repeated slot the last one). Slots out of range are skipped. workspace:
+ * mv_fp8_write_plan_workspace_bytes (0 up to 2048 tokens), rebuilt by every call.
+ */
+size_t mv_fp8_write_plan_workspace_bytes(int64_t num_tokens);
+int mv_fp8_write_plan(const int64_t* slot_mapping, int64_t num_tokens, int32_t block_size,
+                      int64_t num_blocks, const int64_t* positions, int64_t max_positions,
+                      int32_t* items, int32_t* table, int32_t* status, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * Quantising append of one layer's new rows, with the rotary embedding on the
+ * way (cos_table not NULL, as mv_rope_kv_cache_write: query to query_out, key to
+ * the cache and, with key_out, to key_out; without it query and key_out are
+ * NULL and num_q_heads 0). For each touched block, kv head, and K and V apart:
+ *   scale = max(the smallest 2^e >= max|x| / 448 over the call's finite rows in
+ *           the block, e >= -110; the block's scale, unless the call writes place
+ *           0 of the block, which starts it anew);
+ *   the new rows' codes are x / scale rounded to nearest even, NaN where x is
+ *   not finite, |x| limited to 61440 (fp16) or 240 * 2^120 (bf16); where the scale
+ *   grows, the block's other rows are scaled to it, rounded to nearest even.
+ * items, table, plan_status: mv_fp8_write_plan's, over the same num_tokens;
+ * max_items bounds the items it may have found (num_tokens if not known).
+ */
+int mv_fp8_kv_cache_write(
+    const void* query, int64_t q_stride_tok, int64_t q_stride_head, void* query_out,
+    int64_t qo_stride_tok, int64_t qo_stride_head, const void* key, int64_t k_stride_tok,
+    int64_t k_stride_head, void* key_out, int64_t ko_stride_tok, int64_t ko_stride_head,
+    const void* value, int64_t v_stride_tok, int64_t v_stride_head, void* key_cache,
+    void* value_cache, float* kv_scales, const int32_t* items, const int32_t* table,
+    const int32_t* plan_status, int32_t max_items, const int64_t* positions,
+    const void* cos_table, const void* sin_table, int64_t table_stride, int64_t max_positions,
+    int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, int64_t num_blocks, int32_t dtype, void* stream);
+
+/*
+ * Decode attention over the 8-bit pool: mv_paged_decode's arguments, the plan
+ * made by mv_decode_plan with mv_fp8_decode_groups_per_cu; out rows 16-byte
+ * aligned. V codes of places no sequence attends are not used.
+ */
+int mv_fp8_decode_groups_per_cu(int32_t head_dim);
+size_t mv_fp8_paged_decode_workspace_bytes(int32_t num_seqs, int32_t num_q_heads,
+                                           int32_t head_dim, int32_t max_partitions);
+int mv_fp8_paged_decode(const void* query, int64_t q_stride_tok, int64_t q_stride_head,
+                        const void* key_cache, const void* value_cache, const float* kv_scales,
+                        const int32_t* work_items, const int32_t* block_ids,
+                        int64_t block_ids_capacity, int32_t num_work_groups,
+                        int32_t partition_tokens, int32_t max_partitions, int32_t* counters,
+                        void* out, int64_t out_stride_tok, int64_t out_stride_head, float scale,
+                        int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t block_size, int64_t num_blocks, int32_t dtype,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * mv_paged_prefill_blocks over the 8-bit pool (plan and workspace as there): the
+ * prefix's keys are the values its codes stand for, the chunk's the rows given.
+ */
+int mv_fp8_paged_prefill(
+    const void* query, int64_t q_stride_tok, int64_t q_stride_head, const void* key,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* value, int64_t v_stride_tok,
+    int64_t v_stride_head, const void* key_cache, const void* value_cache, const float* kv_scales,
+    const void* block_table, int32_t bt_is_i64, int64_t bt_stride, const int64_t* seqs,
+    int32_t num_seqs, const int32_t* work_items, int32_t num_work_groups, int32_t tokens_per_item,
+    int32_t num_units, int32_t max_parts, void* out, int64_t out_stride_tok,
+    int64_t out_stride_head, float scale, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t block_size, int64_t num_blocks, int32_t dtype, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/*
+ * Gather of cached prefixes from the 8-bit pool: mv_fp8_prefix_slots writes the
+ * pool slot of every prefix token (cu_tokens int64[num_seqs + 1], seq_rows
+ * int64[num_seqs] as mv_gather_paged_kv; -1 where the table has no pool block, counted
+ * in bad int32[1]); mv_fp8_gather_kv reads slots int64[total_tokens] into
+ * out_key / out_value [total_tokens, num_kv_heads, head_dim], code * scale in
+ * dtype (exact), zeros for a slot outside the pool.
+ */
+int mv_fp8_prefix_slots(const void* block_table, int32_t bt_is_i64, int64_t bt_stride,
+                        int32_t bt_rows, int32_t max_blocks, const int64_t* seq_rows,
+                        const int64_t* cu_tokens, int32_t num_seqs, int64_t total_tokens,
+                        int32_t block_size, int64_t num_blocks, int64_t* slots, int32_t* bad,
+                        void* stream);
+int mv_fp8_gather_kv(const void* key_cache, const void* value_cache, const float* kv_scales,
+                     const int64_t* slots, int64_t total_tokens, void* out_key, void* out_value,
+                     int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                     int64_t num_blocks, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

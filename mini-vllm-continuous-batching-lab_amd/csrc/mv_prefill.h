@@ -45,10 +45,14 @@ struct PrefillArgs {
   // an item outside them is skipped, never addressed.
   char* ws;
   int32_t num_units, max_parts;
+  // The pool's scales where it holds 8-bit codes (mv_fp8.h); null otherwise.
+  const float* kv_scales;
 };
 
 // paged_prefill_wide.hip: the 16-bit types with 256 query rows per work group.
 int launch_prefill_wide(const PrefillArgs& a, int head_dim, int dtype, int groups, bool bt_i64, hipStream_t s);
+// fp8_prefill.hip: the same over a pool of 8-bit codes (wide: 256 query rows per work group, else 128).
+int launch_prefill_fp8(const PrefillArgs& a, int head_dim, int dtype, int groups, bool bt_i64, bool wide, hipStream_t s);
 
 namespace {
 

@@ -26,13 +26,13 @@
 // spread over a stage's tiles, four tiles per stage.
 #pragma once
 
+#include "mv_fp8.h"
 #include "mv_prefill.h"
 
 namespace mv {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // A tile of 32 keys keeps p = exp2(s - m) with the row's reference m
 // unchanged while every lane's sum of its keys' p is at most this (every p
@@ -44,11 +44,13 @@ constexpr float kPfFastMax = 4096.f;
 constexpr float kPfStart = -3e38f;
 
 // RW row waves of 32 query rows x SETS key sets that split every stage's
-// tiles; a stage holds T tiles of 32 keys for each set, two stages in LDS.
-template <int DTYPE_, int D_, int RW_, int SETS_>
+// tiles; a stage holds T tiles of 32 keys for each set, two stages in LDS. FP8:
+// the pool holds 8-bit codes (Fp8SubTileCopy).
+template <int DTYPE_, int D_, int RW_, int SETS_, bool FP8_ = false>
 struct Prefill16Traits : TileGeom<DTYPE_, D_> {
   using G = TileGeom<DTYPE_, D_>;
   static constexpr int DTYPE = DTYPE_, D = D_, RW = RW_, SETS = SETS_, T = 2;
+  static constexpr bool kFp8 = FP8_;
   static constexpr int kWaves = RW * SETS;
   static constexpr int kThreads = kWaves * 64;
   static constexpr int kRows = RW * 32;
@@ -64,7 +66,8 @@ struct Prefill16Traits : TileGeom<DTYPE_, D_> {
   static constexpr int kMergeFloats = 32 * 2 + (D / 32) * 16 * 64;
   static constexpr int kMergeBytes = (SETS - 1) * RW * kMergeFloats * 4;
   static constexpr int kIdsOffset = 2 * kStageBytes > kMergeBytes ? 2 * kStageBytes : kMergeBytes;
-  static constexpr int kLdsBytes = kIdsOffset + kPfIdCap * 4;
+  static constexpr int kMixOffset = kIdsOffset + kPfIdCap * 4;  // the codes of one sub-tile
+  static constexpr int kLdsBytes = kMixOffset + (FP8_ ? 2 * kTile * D : 0);
   static_assert(kHalfSubs || kSubs == kWaves, "every wave copies the same amount");
   static_assert(256 % kStageTokens == 0, "parts start at stage boundaries");
   static_assert(kLdsBytes <= 160 * 1024 - 64, "LDS of one work group");
@@ -87,6 +90,113 @@ __device__ __forceinline__ float halves_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// The K/V copies over a pool of 8-bit codes. A sub-tile of 16 prefix keys lies
+// in one pool block (of 16 tokens or more), so it has one K and one V scale. Its
+// codes are copied to LDS as they are, to the first half of their tile, and
+// turned into the tile's 16-bit values in place when the stage lands: the
+// conversion is done once per work group, not by every wave that reads the tile,
+// holds no registers while the copies are in flight (at head_dim 128 there are
+// none left), and what follows is the kernel of a 16-bit pool. Chunk keys are
+// copied as there. Of the one sub-tile across the prefix's end the codes go to
+// an LDS area of their own, and then to the prefix's rows. HALF: a wave
+// copies K (v false) or V only.
+template <int DTYPE, int D, bool HALF>
+struct Fp8SubTile {
+  using B = SubTileCopy<DTYPE, D>;
+  static constexpr int CL = D / 64, NT = HALF ? 1 : 2;
+  static constexpr int kCodeBytes = kTile * D;
+  float scale[NT];
+  int rows;  // prefix rows of the sub-tile in flight
+
+  // Starts the copies of keys kb .. kb + 15 to LDS address dst; returns the loads
+  // of the 16-bit copy whose rows are not to be cleared.
+  __device__ __forceinline__ unsigned fetch(const B& copy, int kb, int win_blk0, uint32_t dst, uint32_t mix,
+                                            int block_id, bool v) {
+    rows = min(max(copy.cached - kb, 0), kTile);
+    if (rows == 0) {
+      if constexpr (HALF) {
+        if (v) return copy.template copy<false, true>(kb, win_blk0, dst, block_id);
+        copy.template copy<true, false>(kb, win_blk0, dst, block_id);
+        return B::kAllValid;  // (only V slots are cleared)
+      } else {
+        return copy.copy(kb, win_blk0, dst, block_id);
+      }
+    }
+    const PrefillArgs& a = copy.a;
+    unsigned valid = B::kAllValid;
+    uint32_t code_dst = dst;
+    int code_step = B::G::kTileBytes;
+    if (rows < kTile) {
+      code_dst = mix;
+      code_step = kCodeBytes;
+      valid = 0;
+      int lane_l = copy.lane;
+      asm volatile("" : "+v"(lane_l));  // (as in the 16-bit copy)
+#pragma unroll
+      for (int c = 0; c < B::L; ++c) {
+        const int j = kb + B::row_of(lane_l, c);
+        const bool ok = j >= copy.cached && j < copy.key_end;
+        const int64_t cr = copy.chunk_row0 + (j - copy.cached);
+        const int64_t off = B::block_of(c) + B::piece_of(lane_l, c);
+        valid |= ok || j < copy.cached ? (1u << c) : 0u;
+        if (!HALF || !v)
+          copy_to_lds_16B((ok ? a.k_new + cr * a.k_st + copy.h * a.k_sh : a.k_cache) + off,
+                          __builtin_amdgcn_readfirstlane(dst + c * 1024));
+        if (!HALF || v)
+          copy_to_lds_16B((ok ? a.v_new + cr * a.v_st + copy.h * a.v_sh : a.v_cache) + off,
+                          __builtin_amdgcn_readfirstlane(dst + B::G::kTileBytes + c * 1024));
+      }
+      if (HALF && !v) valid = B::kAllValid;
+    }
+    const int id = __builtin_amdgcn_readfirstlane(block_id);
+    const bool ok = static_cast<uint32_t>(id) < a.num_blocks_u32;
+    const int64_t bh = (ok ? static_cast<int64_t>(id) : 0) * a.num_kv_heads + copy.h;
+    const int64_t at = ((bh << a.bs_log2) + (kb & ((1 << a.bs_log2) - 1))) * D;
+    // (a scalar load: a vector load's wait would be one for the copies too)
+    const auto* scales = reinterpret_cast<const __attribute__((address_space(4))) float*>(
+        reinterpret_cast<uintptr_t>(a.kv_scales + 2 * bh));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool is_v = HALF ? v : n == 1;
+      scale[n] = ok ? scales[is_v ? 1 : 0] : 0.f;
+#pragma unroll
+      for (int c = 0; c < CL; ++c)
+        copy_to_lds_16B_sv((is_v ? a.v_cache : a.k_cache) + at + c * 1024, copy.lane * 16,
+                           __builtin_amdgcn_readfirstlane(code_dst + (is_v ? code_step : 0) + c * 1024));
+    }
+    return valid;
+  }
+
+  // Turns the landed codes into their rows of the sub-tile at s_sub (an id
+  // outside the pool: zeros).
+  __device__ __forceinline__ void settle(char* s_sub, const char* s_mix, int lane, bool v) const {
+    if (rows == 0) return;
+    asm volatile("" : "+v"(lane));  // (these addresses are not kept through the key loop)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool is_v = HALF ? v : n == 1;
+      char* tile = s_sub + (is_v ? B::G::kTileBytes : 0);
+      const char* from = rows < kTile ? s_mix + (is_v ? kCodeBytes : 0) : tile;
+      u32x4 codes[CL];  // (all read before a row is written over them)
+#pragma unroll
+      for (int c = 0; c < CL; ++c) codes[c] = *reinterpret_cast<const u32x4*>(from + c * 1024 + lane * 16);
+#pragma unroll
+      for (int c = 0; c < CL; ++c) {
+        const int row = (c * 64 + lane) / (D / 16), dim = lane % (D / 16) * 16;
+        u32x2 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = scale[n] > 0.f ? fp8_unpack4<DTYPE>(codes[c][i], scale[n]) : u32x2{0, 0};
+        if (row < rows) {
+          char* at = tile + dim / 64 * 2048 + row * 128;
+          const int piece = dim % 64 / 8, sw = piece_swizzle<8>(row);
+          *reinterpret_cast<u32x4*>(at + ((piece ^ sw) << 4)) = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+          *reinterpret_cast<u32x4*>(at + (((piece + 1) ^ sw) << 4)) = u32x4{w[2][0], w[2][1], w[3][0], w[3][1]};
+        }
+      }
+    }
+  }
+};
 
 template <class Tr, typename BT>
 __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
@@ -228,6 +338,7 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
   // ---- the key stream: this wave's share of stage k's copies into buffer st
   SubTileCopy<DTYPE, D> copy{a, s_ids, h, cached, key_end, chunk_row0, lane, {}, {}, {}};
   copy.init();
+  [[maybe_unused]] Fp8SubTile<DTYPE, D, Tr::kHalfSubs> fp8;
   int win_blk0 = 0;
   const int su = Tr::kHalfSubs ? wave >> 1 : wave;  // the wave's sub-tile
   auto stage_id = [&](int k) __attribute__((always_inline)) {
@@ -236,7 +347,9 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
   auto issue = [&](int k, int st, int id) __attribute__((always_inline)) -> unsigned {
     const int kb = k * Tr::kStageTokens + su * kTile;
     const uint32_t dst = lds0 + st * Tr::kStageBytes + su * Tr::kSubBytes;
-    if constexpr (Tr::kHalfSubs) {
+    if constexpr (Tr::kFp8) {
+      return fp8.fetch(copy, kb, win_blk0, dst, lds0 + Tr::kMixOffset, id, Tr::kHalfSubs && (wave & 1));
+    } else if constexpr (Tr::kHalfSubs) {
       if (wave & 1) return copy.template copy<false, true>(kb, win_blk0, dst, id);
       copy.template copy<true, false>(kb, win_blk0, dst, id);
       return copy.kAllValid;  // (only V slots are cleared)
@@ -250,8 +363,12 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
   // loaded read pool row 0 instead: they are cleared first (P is 0 there, but
   // 0 * NaN would not be).
   auto land = [&](int st, unsigned ok, bool more) __attribute__((always_inline)) {
-    wait_vmcnt_groups<Tr::kWaveLoads, 1>(more);
+    if constexpr (Tr::kFp8) wait_vmcnt<0>();  // (one stage in flight)
+    else wait_vmcnt_groups<Tr::kWaveLoads, 1>(more);
     asm volatile("" ::: "memory");
+    if constexpr (Tr::kFp8)
+      fp8.settle(s_lds + st * Tr::kStageBytes + su * Tr::kSubBytes, s_lds + Tr::kMixOffset, lane,
+                 Tr::kHalfSubs && (wave & 1));
     if (__builtin_amdgcn_ballot_w64(ok != copy.kAllValid) != 0) {
       char* vdst = s_lds + st * Tr::kStageBytes + su * Tr::kSubBytes + Tr::kTileBytes;
 #pragma unroll
@@ -330,8 +447,9 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
     const int ns = (min(key_end, win0 + win_tokens) - first + Tr::kStageTokens - 1) / Tr::kStageTokens;
     const unsigned ok = issue(k0, 0, stage_id(k0));
     unsigned ok_next = 0;
-    if (ns > 1) ok_next = issue(k0 + 1, 1, stage_id(k0 + 1));
+    if (!Tr::kFp8 && ns > 1) ok_next = issue(k0 + 1, 1, stage_id(k0 + 1));
     land(0, ok, ns > 1);
+    if (Tr::kFp8 && ns > 1) ok_next = issue(k0 + 1, 1, stage_id(k0 + 1));
 
     // this wave's tiles that some row of it sees, and the stages full of them
     const int set_key = first + set * 32;

@@ -624,7 +624,7 @@ int paged_prefill(const void* query, int64_t q_stride_tok, int64_t q_stride_head
                   void* out, int64_t out_stride_tok, int64_t out_stride_head, float scale,
                   int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                   int32_t block_size, int64_t num_blocks, int32_t dtype,
-                  const PrefillParts* parts, void* stream) {
+                  const PrefillParts* parts, void* stream, const float* kv_scales = nullptr) {
   const int eb = dtype_bytes(dtype);
   if (eb == 0) return fail(MV_ERR_UNSUPPORTED, "mv_paged_prefill: unknown dtype %d", dtype);
   if (head_dim != 64 && head_dim != 128)
@@ -684,6 +684,7 @@ int paged_prefill(const void* query, int64_t q_stride_tok, int64_t q_stride_head
   }
   a.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (out_stride_tok * eb) % 16 == 0 &&
               (out_stride_head * eb) % 16 == 0;
+  a.kv_scales = kv_scales;
   a.item_ints = 4;
   a.ws = nullptr;
   a.num_units = 0;
@@ -710,6 +711,8 @@ int paged_prefill(const void* query, int64_t q_stride_tok, int64_t q_stride_head
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool i64 = bt_is_i64 != 0;
+  if (kv_scales)
+    return launch_prefill_fp8(a, head_dim, dtype, num_work_groups, i64, tokens_per_item * n_rep > 128, s);
   if (dtype != MV_DTYPE_F32 && tokens_per_item * n_rep > 128)
     return launch_prefill_wide(a, head_dim, dtype, num_work_groups, i64, s);
   switch (dtype) {
@@ -777,4 +780,32 @@ extern "C" int mv_paged_prefill_blocks(
                            tokens_per_item, out, out_stride_tok, out_stride_head, scale, num_q_heads,
                            num_kv_heads, head_dim, block_size, num_blocks, dtype,
                            max_parts > 1 ? &parts : nullptr, stream);
+}
+
+extern "C" int mv_fp8_paged_prefill(
+    const void* query, int64_t q_stride_tok, int64_t q_stride_head, const void* key,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* value, int64_t v_stride_tok,
+    int64_t v_stride_head, const void* key_cache, const void* value_cache, const float* kv_scales,
+    const void* block_table, int32_t bt_is_i64, int64_t bt_stride, const int64_t* seqs,
+    int32_t num_seqs, const int32_t* work_items, int32_t num_work_groups, int32_t tokens_per_item,
+    int32_t num_units, int32_t max_parts, void* out, int64_t out_stride_tok,
+    int64_t out_stride_head, float scale, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t block_size, int64_t num_blocks, int32_t dtype, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  if (dtype != MV_DTYPE_F16 && dtype != MV_DTYPE_BF16)
+    return mv::fail(MV_ERR_UNSUPPORTED, "mv_fp8_paged_prefill: dtype %d (fp16 or bf16 rows)", dtype);
+  if (!mv::is_pow2(block_size) || block_size < 16 || block_size > 256)
+    return mv::fail(MV_ERR_UNSUPPORTED, "mv_fp8_paged_prefill: block_size %d (a power of two from 16 to 256)",
+                    block_size);
+  if (tokens_per_item <= 0)
+    return mv::fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_paged_prefill: %d tokens per item", tokens_per_item);
+  if (!kv_scales || reinterpret_cast<uintptr_t>(kv_scales) % 8)
+    return mv::fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_paged_prefill: scales null or not 8-byte aligned");
+  const mv::PrefillParts parts{num_units, max_parts, workspace, workspace_bytes};
+  return mv::paged_prefill(query, q_stride_tok, q_stride_head, key, k_stride_tok, k_stride_head,
+                           value, v_stride_tok, v_stride_head, key_cache, value_cache, block_table,
+                           bt_is_i64, bt_stride, seqs, num_seqs, work_items, num_work_groups,
+                           tokens_per_item, out, out_stride_tok, out_stride_head, scale, num_q_heads,
+                           num_kv_heads, head_dim, block_size, num_blocks, dtype,
+                           max_parts > 1 ? &parts : nullptr, stream, kv_scales);
 }

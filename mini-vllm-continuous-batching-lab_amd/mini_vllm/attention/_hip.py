@@ -47,6 +47,11 @@ MV_PLAN_PARTITION_TOKENS = 6
 MV_PLAN_IDS_PER_ITEM = 7
 MV_PLAN_WORDS = 8
 MV_DECODE_SCRATCH_BYTES = 16 << 20
+MV_FP8_PLAN_OUT_OF_RANGE = 0
+MV_FP8_PLAN_REPEATED = 1
+MV_FP8_PLAN_POSITIONS = 2
+MV_FP8_PLAN_ITEMS = 3
+MV_FP8_PLAN_WORDS = 4
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 DEFAULT_LIB_PATH = os.path.join(_PKG_ROOT, "lib", "libmvattn.so")
@@ -214,6 +219,60 @@ SIGNATURES = {
         _F, _I32, _I32, _I32,      # scale, num_q_heads, num_kv_heads, head_dim
         _I32, _I64, _I32,          # block_size, num_blocks, dtype
         _P, ctypes.c_size_t, _P,   # workspace, workspace_bytes, stream
+    ]),
+    # the 8-bit KV cache
+    "mv_fp8_write_plan_workspace_bytes": (_SZ, [_I64]),
+    "mv_fp8_write_plan": (ctypes.c_int, [
+        _P, _I64, _I32, _I64,      # slot_mapping, num_tokens, block_size, num_blocks
+        _P, _I64, _P, _P, _P,      # positions, max_positions, items, table, status
+        _P, _SZ, _P,               # workspace, workspace_bytes, stream
+    ]),
+    "mv_fp8_kv_cache_write": (ctypes.c_int, [
+        _P, _I64, _I64,            # query, strides
+        _P, _I64, _I64,            # query_out, strides
+        _P, _I64, _I64,            # key, strides
+        _P, _I64, _I64,            # key_out, strides
+        _P, _I64, _I64,            # value, strides
+        _P, _P, _P,                # key_cache, value_cache, kv_scales
+        _P, _P, _P, _I32,          # items, table, plan_status, max_items
+        _P, _P, _P, _I64, _I64,    # positions, cos, sin, table_stride, max_positions
+        _I64, _I32, _I32, _I32,    # num_tokens, num_q_heads, num_kv_heads, head_dim
+        _I32, _I64, _I32, _P,      # block_size, num_blocks, dtype, stream
+    ]),
+    "mv_fp8_decode_groups_per_cu": (ctypes.c_int, [_I32]),
+    "mv_fp8_paged_decode_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
+    "mv_fp8_paged_decode": (ctypes.c_int, [
+        _P, _I64, _I64,            # query, strides
+        _P, _P, _P,                # key_cache, value_cache, kv_scales
+        _P, _P, _I64, _I32,        # work_items, block_ids, block_ids_capacity, num_work_groups
+        _I32, _I32, _P,            # partition_tokens, max_partitions, counters
+        _P, _I64, _I64,            # out, strides
+        _F, _I32, _I32, _I32, _I32,  # scale, num_seqs, num_q_heads, num_kv_heads, head_dim
+        _I32, _I64, _I32,          # block_size, num_blocks, dtype
+        _P, _SZ, _P,               # workspace, workspace_bytes, stream
+    ]),
+    "mv_fp8_paged_prefill": (ctypes.c_int, [
+        _P, _I64, _I64,            # query, strides
+        _P, _I64, _I64,            # key, strides
+        _P, _I64, _I64,            # value, strides
+        _P, _P, _P,                # key_cache, value_cache, kv_scales
+        _P, _I32, _I64,            # block_table, bt_is_i64, bt_stride
+        _P, _I32, _P, _I32,        # seqs, num_seqs, work_items, num_work_groups
+        _I32, _I32, _I32,          # tokens_per_item, num_units, max_parts
+        _P, _I64, _I64,            # out, strides
+        _F, _I32, _I32, _I32,      # scale, num_q_heads, num_kv_heads, head_dim
+        _I32, _I64, _I32,          # block_size, num_blocks, dtype
+        _P, _SZ, _P,               # workspace, workspace_bytes, stream
+    ]),
+    "mv_fp8_prefix_slots": (ctypes.c_int, [
+        _P, _I32, _I64, _I32, _I32,  # block_table, bt_is_i64, bt_stride, bt_rows, max_blocks
+        _P, _P, _I32, _I64,        # seq_rows, cu_tokens, num_seqs, total_tokens
+        _I32, _I64, _P, _P, _P,    # block_size, num_blocks, slots, bad, stream
+    ]),
+    "mv_fp8_gather_kv": (ctypes.c_int, [
+        _P, _P, _P, _P, _I64,      # key_cache, value_cache, kv_scales, slots, total_tokens
+        _P, _P, _I32, _I32,        # out_key, out_value, num_kv_heads, head_dim
+        _I32, _I64, _I32, _P,      # block_size, num_blocks, dtype, stream
     ]),
 }
 

@@ -236,7 +236,7 @@ def clear_deferred(capture_id: Optional[int] = None) -> None:
 
 # The eager (not captured) per-step checks and plans that _cache_get keeps.
 _EAGER_CACHES = ("slots", "fused", "plan", "fused_step", "rope_step", "write_step", "rope_rows",
-                 "positions", "prefill")
+                 "positions", "prefill", "fp8_write", "fp8_decode", "fp8_prefill")
 
 
 def invalidate_cached_metadata() -> None:
@@ -484,7 +484,9 @@ def _groups_per_cu(device: torch.device, head_dim: int, dtype: torch.dtype) -> T
     if split is None:
         cus = torch.cuda.get_device_properties(device).multi_processor_count
         per_cu = os.environ.get("MVATTN_GROUPS_PER_CU")
-        if per_cu is None:
+        if per_cu is None and dtype is torch.float8_e4m3fn:
+            per_cu = _hip.load().mv_fp8_decode_groups_per_cu(head_dim)
+        elif per_cu is None:
             per_cu = _hip.load().mv_decode_groups_per_cu(head_dim, _hip.MV_DTYPE[dtype])
         split = _SPLIT[key] = (max(1, int(per_cu)), cus)
     return split
@@ -1677,12 +1679,21 @@ def _prefill_plan(block_table, rows, cached, qlens, block_size, num_blocks, num_
     workspace for the merge (counters zero). ``MVATTN_PREFILL_PARTS`` caps
     the parts per unit (1: no cut).
     """
-    lib = _hip.load()
     extra = (tuple(rows), tuple(cached), tuple(qlens), block_size, num_blocks, num_q_heads,
              num_kv_heads, head_dim, dtype, device)
     hit = _cache_get("prefill", (block_table,), extra)
     if hit is not None:
         return hit
+    plan = _prefill_plan_make(block_table, rows, cached, qlens, block_size, num_blocks, num_q_heads,
+                              num_kv_heads, head_dim, dtype, device)
+    _cache_put("prefill", (block_table,), extra, plan)
+    return plan
+
+
+def _prefill_plan_make(block_table, rows, cached, qlens, block_size, num_blocks, num_q_heads,
+                       num_kv_heads, head_dim, dtype, device):
+    """``_prefill_plan``, made anew."""
+    lib = _hip.load()
     # a negative chunk would shift the rows of the sequences after it out of
     # the tensors; a negative prefix hides the chunk's own first keys
     for r, c, q in zip(rows, cached, qlens):
@@ -1741,7 +1752,6 @@ def _prefill_plan(block_table, rows, cached, qlens, block_size, num_blocks, num_
         _ptr(meta), len(rows), _ptr(work), work.shape[0], tokens, units, max_parts,
         float(head_dim ** -0.5), num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
         _hip.MV_DTYPE[dtype], _ptr(ws), ws.numel() if ws is not None else 0, device.index),)
-    _cache_put("prefill", (block_table,), extra, plan)
     return plan
 
 
@@ -1999,15 +2009,30 @@ class AttentionBackendGPU(AttentionBackend):
         head_dim: int,
         dtype: torch.dtype,
         device: torch.device,
+        cache_dtype: Optional[torch.dtype] = None,
     ) -> KVCachePool:
+        """``cache_dtype=torch.float8_e4m3fn``: an 8-bit pool with a scale per
+        block and kv head (``paged_attention_fp8``); every method of the backend
+        works on it. Default: ``dtype``."""
         if not _is_pow2(block_size):
             raise RuntimeError(
                 f"AttentionBackendGPU: block_size={block_size} must be a positive power of 2."
             )
         if dtype not in SUPPORTED_DTYPES:
             raise RuntimeError(f"AttentionBackendGPU: dtype {dtype} not supported")
+        if cache_dtype not in (None, dtype, _fp8.FP8_DTYPE):
+            raise RuntimeError(f"AttentionBackendGPU: cache_dtype {cache_dtype} not supported "
+                               f"({dtype} or {_fp8.FP8_DTYPE})")
+        if cache_dtype is _fp8.FP8_DTYPE and (dtype not in _fp8.FP8_ROW_DTYPES
+                                              or block_size not in _fp8.FP8_BLOCK_SIZES):
+            raise RuntimeError(
+                f"AttentionBackendGPU: an 8-bit cache of {dtype} rows in blocks of {block_size} is "
+                f"not supported (fp16 or bf16, a power of 2 from 16 to 256)"
+            )
+        # (another package's pool class knows no cache_dtype)
+        held = {} if cache_dtype in (None, dtype) else {"cache_dtype": cache_dtype}
         pool = KVCachePool.allocate(
-            num_layers, num_blocks, block_size, num_kv_heads, head_dim, dtype, device
+            num_layers, num_blocks, block_size, num_kv_heads, head_dim, dtype, device, **held
         )
         self._pool = pool
         self._block_size = block_size
@@ -2022,6 +2047,12 @@ class AttentionBackendGPU(AttentionBackend):
     ) -> None:
         pool = self._pool
         assert pool is not None, "allocate_pool must be called first"
+        if getattr(pool, "kv_scales", None) is not None:
+            _fp8.hip_fp8_cache_write(
+                key, value, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
+                pool.kv_scales[layer_idx], slot_mapping, pool.block_size,
+            )
+            return
         hip_cache_write(
             key, value, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
             slot_mapping, pool.block_size,
@@ -2046,6 +2077,12 @@ class AttentionBackendGPU(AttentionBackend):
         chunk's attention reads it)."""
         pool = self._pool
         assert pool is not None, "allocate_pool must be called first"
+        if getattr(pool, "kv_scales", None) is not None:
+            return _fp8.hip_fp8_rope_kv_cache_write(
+                query, key, value, positions, rope.cos, rope.sin, pool.key_caches[layer_idx],
+                pool.value_caches[layer_idx], pool.kv_scales[layer_idx], slot_mapping,
+                pool.block_size, return_key=return_key,
+            )
         return hip_rope_kv_cache_write(
             query, key, value, positions, rope.cos, rope.sin,
             pool.key_caches[layer_idx], pool.value_caches[layer_idx], slot_mapping,
@@ -2066,6 +2103,12 @@ class AttentionBackendGPU(AttentionBackend):
             return query
         # Rows of decode_block_tables are decode sequences 0..B-1 in query
         # order (the runner rebases seq_indices, qwen_runner.py:213-251).
+        if getattr(pool, "kv_scales", None) is not None:
+            return _fp8.hip_fp8_decode_attention(
+                query, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
+                pool.kv_scales[layer_idx], attn_metadata.decode_block_tables, group.kv_len_after,
+                pool.block_size,
+            )
         return hip_decode_attention(
             query, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
             attn_metadata.decode_block_tables, group.kv_len_after, pool.block_size,
@@ -2097,6 +2140,9 @@ class AttentionBackendGPU(AttentionBackend):
         if group is None:
             self.write_kv_cache(layer_idx, key, value, slot_mapping)
             return query
+        if getattr(pool, "kv_scales", None) is not None:  # (two launches)
+            self.write_kv_cache(layer_idx, key, value, slot_mapping)
+            return self.decode_attention(layer_idx, query, attn_metadata, pool)
         return hip_decode_attention(
             query, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
             attn_metadata.decode_block_tables, group.kv_len_after, pool.block_size,
@@ -2129,6 +2175,10 @@ class AttentionBackendGPU(AttentionBackend):
         if group is None:
             self.rope_write_kv_cache(layer_idx, query, key, value, positions, rope, slot_mapping)
             return query
+        if getattr(pool, "kv_scales", None) is not None:  # (two launches)
+            query, _ = self.rope_write_kv_cache(layer_idx, query, key, value, positions, rope,
+                                                slot_mapping)
+            return self.decode_attention(layer_idx, query, attn_metadata, pool)
         return hip_decode_attention(
             query, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
             attn_metadata.decode_block_tables, group.kv_len_after, pool.block_size,
@@ -2168,7 +2218,16 @@ class AttentionBackendGPU(AttentionBackend):
         else:
             cached = torch.cat([g.cached_len_before.reshape(-1) for g in groups])
             qlens = torch.cat([g.query_len.reshape(-1) for g in groups])
+        if getattr(pool, "kv_scales", None) is not None:
+            return _fp8.hip_fp8_prefill_attention(
+                query, key, value, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
+                pool.kv_scales[layer_idx], attn_metadata.prefill_block_tables, rows, cached, qlens,
+                pool.block_size,
+            )
         return hip_prefill_attention(
             query, key, value, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
             attn_metadata.prefill_block_tables, rows, cached, qlens, pool.block_size,
         )
+
+
+from . import paged_attention_fp8 as _fp8  # noqa: E402  (uses this module's plans and checks)

@@ -26,6 +26,14 @@ def _default_device() -> torch.device:
     return torch.device("cuda" if torch.cuda.is_available() else "cpu")
 
 
+def _block_bytes(num_kv_heads: int, block_size: int, head_dim: int, dtype: torch.dtype,
+                 cache_dtype: Optional[torch.dtype]) -> int:
+    """K plus V bytes of one block in one layer, of 8-bit codes with their scales."""
+    held = dtype if cache_dtype is None else cache_dtype
+    values = 2 * num_kv_heads * block_size * head_dim * torch.empty((), dtype=held).element_size()
+    return values + (2 * num_kv_heads * 4 if held is torch.float8_e4m3fn else 0)
+
+
 @dataclass
 class KVCachePool:
     key_caches: List[torch.Tensor]
@@ -37,6 +45,10 @@ class KVCachePool:
     head_dim: int
     device: torch.device
     dtype: torch.dtype
+    # An 8-bit pool (``key_caches`` / ``value_caches`` of float8_e4m3fn): per layer
+    # the fp32 scales ``[num_blocks, num_kv_heads, 2]`` (K's, V's), zero for a block
+    # never written. None: the caches hold ``dtype``.
+    kv_scales: Optional[List[torch.Tensor]] = None
 
     @staticmethod
     def allocate(
@@ -47,9 +59,11 @@ class KVCachePool:
         head_dim: int,
         dtype: torch.dtype = torch.float16,
         device: Optional[torch.device] = None,
+        cache_dtype: Optional[torch.dtype] = None,
     ) -> "KVCachePool":
         """Allocate uninitialised per-layer K/V tensors (reference pool.py:64-114).
 
+        ``cache_dtype=torch.float8_e4m3fn``: 8-bit codes, with the scales (zeroed).
         Raises ``ValueError`` naming the first non-positive size.
         """
         for name, value in (
@@ -63,10 +77,16 @@ class KVCachePool:
                 raise ValueError(f"{name} must be > 0, got {value}")
         dev = torch.device(device) if device is not None else _default_device()
         shape = (num_blocks, num_kv_heads, block_size, head_dim)
-        keys = [torch.empty(shape, dtype=dtype, device=dev) for _ in range(num_layers)]
-        values = [torch.empty(shape, dtype=dtype, device=dev) for _ in range(num_layers)]
+        held = dtype if cache_dtype is None else cache_dtype
+        if held not in (dtype, torch.float8_e4m3fn):
+            raise ValueError(f"cache_dtype must be {dtype} or torch.float8_e4m3fn, got {held}")
+        keys = [torch.empty(shape, dtype=held, device=dev) for _ in range(num_layers)]
+        values = [torch.empty(shape, dtype=held, device=dev) for _ in range(num_layers)]
+        scales = None
+        if held is torch.float8_e4m3fn:
+            scales = [torch.zeros(num_blocks, num_kv_heads, 2, device=dev) for _ in range(num_layers)]
         return KVCachePool(keys, values, num_blocks, block_size, num_layers,
-                           num_kv_heads, head_dim, dev, dtype)
+                           num_kv_heads, head_dim, dev, dtype, scales)
 
     def get_key_cache(self, layer_idx: int) -> torch.Tensor:
         return self.key_caches[layer_idx]
@@ -75,8 +95,8 @@ class KVCachePool:
         return self.value_caches[layer_idx]
 
     def reset(self) -> None:
-        """Zero every layer's K and V."""
-        for t in (*self.key_caches, *self.value_caches):
+        """Zero every layer's K and V (and scales)."""
+        for t in (*self.key_caches, *self.value_caches, *(self.kv_scales or ())):
             t.zero_()
 
     @property
@@ -86,9 +106,9 @@ class KVCachePool:
 
     @property
     def bytes_per_block_per_layer(self) -> int:
-        """K plus V bytes of one block in one layer."""
-        itemsize = torch.empty((), dtype=self.dtype).element_size()
-        return 2 * self.num_kv_heads * self.block_size * self.head_dim * itemsize
+        """K plus V bytes (and scales) of one block in one layer."""
+        return _block_bytes(self.num_kv_heads, self.block_size, self.head_dim, self.dtype,
+                            torch.float8_e4m3fn if self.kv_scales is not None else None)
 
     @property
     def bytes_per_block_total(self) -> int:
@@ -110,6 +130,7 @@ def compute_num_gpu_blocks(
     peak_runtime_estimate: int = 0,
     workspace_reserve: int = _WORKSPACE_RESERVE,
     num_gpu_blocks_override: Optional[int] = None,
+    cache_dtype: Optional[torch.dtype] = None,
 ) -> int:
     """Number of pool blocks that fit in free device memory.
 
@@ -119,7 +140,8 @@ def compute_num_gpu_blocks(
     bytes of one block across all layers; never below ``MIN_BLOCKS``. On a
     CPU device it returns ``MIN_BLOCKS``. On one MI355X (288 GB HBM3E) the
     Qwen2-0.5B pool (24 layers, 2 kv heads, head_dim 64, block 16, bf16:
-    196608 bytes per block) holds about 1.3 M blocks, i.e. 21 M tokens.
+    196608 bytes per block) holds about 1.3 M blocks, i.e. 21 M tokens;
+    with ``cache_dtype=torch.float8_e4m3fn`` (98688 bytes) twice that.
     """
     if not 0 < gpu_memory_utilization <= 1.0:
         raise ValueError(
@@ -141,6 +163,5 @@ def compute_num_gpu_blocks(
             f"GPU memory exhausted after deductions: free={free_bytes}, "
             f"peak={peak_runtime_estimate}, workspace={workspace_reserve}"
         )
-    itemsize = torch.empty((), dtype=dtype).element_size()
-    per_block = num_layers * 2 * num_kv_heads * block_size * head_dim * itemsize
+    per_block = num_layers * _block_bytes(num_kv_heads, block_size, head_dim, dtype, cache_dtype)
     return max(MIN_BLOCKS, int(usable * gpu_memory_utilization) // per_block)
