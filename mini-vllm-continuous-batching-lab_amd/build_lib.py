@@ -117,29 +117,34 @@ def build_launcher(verbose: bool = False) -> str:
     return out
 
 
-TORCH_CALLS_SOURCE = os.path.join(CSRC, "py_torch.cpp")
+TORCH_CALLS = {"_mvtorch": "py_torch.cpp", "_mvfp8": "py_fp8.cpp"}
 
 
 def build_torch_calls(verbose: bool = False) -> str:
-    """Compile the native per-layer launches (``csrc/py_torch.cpp``, host C++
-    on torch's headers) into ``mini_vllm/attention/_mvtorch<EXT_SUFFIX>``;
-    returns its path. Without it the Python wrappers do the same work."""
+    """Compile the native per-layer launches (``csrc/py_torch.cpp``,
+    ``csrc/py_fp8.cpp``, host C++ on torch's headers) into
+    ``mini_vllm/attention/_mvtorch<EXT_SUFFIX>`` and ``_mvfp8``; returns the
+    paths. Without them the Python wrappers do the same work."""
+    return " ".join(_build_torch_call(name, src, verbose) for name, src in TORCH_CALLS.items())
+
+
+def _build_torch_call(name: str, source: str, verbose: bool) -> str:
     import sysconfig
 
     import torch
 
-    out = os.path.join(LAUNCHER_DIR, "_mvtorch" + sysconfig.get_config_var("EXT_SUFFIX"))
+    out = os.path.join(LAUNCHER_DIR, name + sysconfig.get_config_var("EXT_SUFFIX"))
     cxx = shutil.which("g++") or shutil.which("c++")
     if not cxx:
         raise RuntimeError("no C++ compiler (g++) for the per-layer launches")
     root = os.path.dirname(torch.__file__)
-    fd, tmp = tempfile.mkstemp(prefix="_mvtorch.", suffix=".so.tmp", dir=LAUNCHER_DIR)
+    fd, tmp = tempfile.mkstemp(prefix=name + ".", suffix=".so.tmp", dir=LAUNCHER_DIR)
     os.close(fd)
     cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", os.path.join(root, "include"), "-I", sysconfig.get_paths()["include"],
-           "-I", INCLUDE, TORCH_CALLS_SOURCE, "-o", tmp, "-L", os.path.join(root, "lib"),
-           "-ltorch_python", "-ltorch_cpu", "-lc10"]
+           "-I", INCLUDE, "-I", CSRC, os.path.join(CSRC, source), "-o", tmp,
+           "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)

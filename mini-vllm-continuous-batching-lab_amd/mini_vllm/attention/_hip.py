@@ -307,6 +307,10 @@ decode_write_step = None
 native = None
 launcher = None
 
+# _mvfp8 (csrc/py_fp8.cpp), bound likewise: the calls of the 8-bit cache from a
+# plan's packed words. None where it is not built.
+native_fp8 = None
+
 # The step words' layout (csrc/py_launch.c): mv_paged_decode_write's
 # step-constant arguments in its order, one little-endian 64-bit word each,
 # the scale as a double.
@@ -331,6 +335,11 @@ def step_words(slots: int, rope_cos: int, rope_sin: int, work: int, ids: int, id
 # for prefill the device index.
 _DECODE_WORDS = struct.Struct("<7qd9q")
 _PREFILL_WORDS = struct.Struct("<10qd9q")
+# _mvfp8's: write's, decode's (mv_paged_decode's and the device index), gather's
+# (prefill's are _mvtorch.prefill's).
+_FP8_WRITE_WORDS = struct.Struct("<10q")
+_FP8_DECODE_WORDS = struct.Struct("<7qd10q")
+_FP8_GATHER_WORDS = struct.Struct("<5q")
 
 
 def decode_words(*args) -> bytes:
@@ -343,6 +352,38 @@ def prefill_words(block_table, *args) -> bytes:
     workspace, last but two, None if there are none)."""
     return _PREFILL_WORDS.pack(block_table or 0, *args[:-3], args[-3] or 0, args[-2],
                                args[-1] or 0)
+
+
+def fp8_write_words(*args) -> bytes:
+    """Items, table, status, the most items, positions (None: not checked),
+    tokens, block size, blocks, table rows, device index."""
+    return _FP8_WRITE_WORDS.pack(*args[:4], args[4] or 0, *args[5:])
+
+
+def fp8_decode_words(*args) -> bytes:
+    """mv_paged_decode's (the workspace None if there is none) and the device
+    index."""
+    return _FP8_DECODE_WORDS.pack(*args[:-3], args[-3] or 0, *args[-2:])
+
+
+def fp8_gather_words(*args) -> bytes:
+    """Slots, tokens, block size, blocks, device index."""
+    return _FP8_GATHER_WORDS.pack(*args)
+
+
+def _bind_fp8(lib: ctypes.CDLL) -> None:
+    global native_fp8
+    native_fp8 = None
+    try:
+        from . import _mvfp8
+    except ImportError:
+        return
+    if _mvfp8.ABI != ABI_VERSION:
+        return
+    _mvfp8.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+        lib.mv_fp8_kv_cache_write, lib.mv_fp8_paged_decode, lib.mv_fp8_paged_prefill,
+        lib.mv_fp8_gather_kv)))
+    native_fp8 = _mvfp8
 
 
 def _bind_native(lib: ctypes.CDLL, mvlaunch) -> None:
@@ -424,6 +465,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
             )
         if path is None:
             _bind_calls(lib)
+            _bind_fp8(lib)
             _lib = lib
         return lib
 

@@ -90,6 +90,7 @@ class _Plan:
     buffers: Tuple[torch.Tensor, ...]
     stream: int = 0
     capture: int = 0
+    words: Optional[bytes] = None  # for the native calls (on the plan's own stream)
 
     def _used(self, raw_stream: int) -> None:
         """The buffers' memory is not reused before this call is done, where it
@@ -98,6 +99,15 @@ class _Plan:
             current = torch.cuda.current_stream(self.device)
             for t in self.buffers:
                 t.record_stream(current)
+
+
+def _seen_plan(name: str, *tensors):
+    """The plan that an earlier layer of this eager step made for these, unmodified,
+    metadata tensors, looked up natively (None: not known here)."""
+    entry, lookup = getattr(_gpu._state, name, None), _hip.native
+    if entry is None or lookup is None or not lookup.seen(entry[0].refs, entry[0].versions, *tensors):
+        return None
+    return None if _gpu._capturing() else entry[1]
 
 
 def _check_pool(key_cache: torch.Tensor, value_cache: torch.Tensor, kv_scales: torch.Tensor,
@@ -225,6 +235,9 @@ def plan_fp8_write(
             st = status.tolist()
             raise_write(st)
             plan.max_items = st[_hip.MV_FP8_PLAN_ITEMS]
+        plan.words = _hip.fp8_write_words(
+            base + 4 * _hip.MV_FP8_PLAN_WORDS, table_at, base, plan.max_items, _gpu._ptr(pos), n,
+            block_size, num_blocks, plan.max_positions, device.index)
     return plan
 
 
@@ -243,6 +256,19 @@ def _write_plan(slot_mapping, block_size, num_blocks, device, positions, max_pos
 
 def _append(who, query, key, value, positions, cos, sin, key_cache, value_cache, kv_scales,
             slot_mapping, block_size, return_key, plan):
+    native = _hip.native_fp8
+    known = plan
+    if known is None:
+        known = _seen_plan("fp8_write", *((slot_mapping,) if cos is None else (slot_mapping, positions)))
+    if known is not None and native is not None and slot_mapping.shape == (known.num_tokens,):
+        stream = _gpu._stream(known.device)
+        if stream == known.stream and (cos is None or known.max_positions):
+            done = native.write(known.words, query, key, value, cos, sin, key_cache, value_cache,
+                                kv_scales, block_size, return_key, stream)
+            if done is not None:
+                if type(done) is int:
+                    _hip.check(done, "mv_fp8_kv_cache_write")
+                return done
     num_blocks, num_kv_heads, head_dim = _check_pool(key_cache, value_cache, kv_scales, block_size, who)
     device, dtype = key_cache.device, key.dtype
     num_tokens = key.shape[0]
@@ -461,6 +487,17 @@ def hip_fp8_decode_attention(
     rounded to the query's type for the product with V. Errors as there;
     ``plan``: ``plan_fp8_decode`` of this table and these lengths.
     """
+    native = _hip.native_fp8
+    known = plan if plan is not None else _seen_plan("fp8_decode", block_table, kv_len_after)
+    if known is not None and native is not None and known.words is not None:
+        stream = _gpu._stream(known.device)
+        if stream == known.stream:
+            output = native.decode(known.words, query, key_cache, value_cache, kv_scales, block_table,
+                                   kv_len_after, block_size, stream)
+            if output is not None:
+                if type(output) is int:
+                    _hip.check(output, "mv_fp8_paged_decode")
+                return output
     num_blocks, num_kv_heads, head_dim = _check_pool(key_cache, value_cache, kv_scales, block_size,
                                                      "hip_fp8_decode_attention")
     num_seqs, num_q_heads, q_dim = query.shape
@@ -500,17 +537,20 @@ def hip_fp8_decode_attention(
         ws = plan.workspace(num_q_heads, head_dim)
         query, qp, q_st, q_sh = _gpu._row_args(query)
         o_st, o_sh, _ = output.stride()
+        split = (p.work.data_ptr(), p.block_ids.data_ptr(), p.block_ids.numel(), p.num_groups,
+                 p.partition_tokens, p.max_parts, p.counters.data_ptr())
+        shape = (float(head_dim ** -0.5), num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+                 num_blocks, _hip.MV_DTYPE[dtype])
+        space = (_gpu._ptr(ws), ws.numel() if ws is not None else 0)
         _hip.check(
             _hip.load().mv_fp8_paged_decode(
                 qp, q_st, q_sh, key_cache.data_ptr(), value_cache.data_ptr(), kv_scales.data_ptr(),
-                p.work.data_ptr(), p.block_ids.data_ptr(), p.block_ids.numel(), p.num_groups,
-                p.partition_tokens, p.max_parts, p.counters.data_ptr(), output.data_ptr(), o_st,
-                o_sh, float(head_dim ** -0.5), num_seqs, num_q_heads, num_kv_heads, head_dim,
-                block_size, num_blocks, _hip.MV_DTYPE[dtype], _gpu._ptr(ws),
-                ws.numel() if ws is not None else 0, stream,
+                *split, output.data_ptr(), o_st, o_sh, *shape, *space, stream,
             ),
             "mv_fp8_paged_decode",
         )
+        # the step's other layers (the same query heads) launch from these words
+        plan.words = _hip.fp8_decode_words(*split, *shape, *space, device.index)
     return output
 
 
@@ -565,8 +605,21 @@ def plan_fp8_prefill(
         torch.cuda.current_stream(device).synchronize()  # (complete, for whatever stream uses it)
         return Fp8PrefillPlan(
             device, tuple(t for t in (bt, meta, work, ws) if t is not None), _gpu._stream(device),
-            plan=made, num_seqs=len(rows), total=sum(qlens),
+            words=made[8], plan=made, num_seqs=len(rows), total=sum(qlens),
             key=(block_size, num_blocks, num_q_heads, num_kv_heads, head_dim, dtype))
+
+
+def _prefill_native(plan, query, key, value, key_cache, value_cache, kv_scales, block_size):
+    """The call's checks and launch in native code (None: not the plain case)."""
+    native = _hip.native_fp8
+    stream = _gpu._stream(plan.device)
+    if native is None or stream != plan.stream:
+        return None
+    out = native.prefill(plan.words, query, key, value, key_cache, value_cache, kv_scales, plan.total,
+                         block_size, stream)
+    if type(out) is int:
+        _hip.check(out, "mv_fp8_paged_prefill")
+    return out
 
 
 def hip_fp8_prefill_attention(
@@ -589,6 +642,10 @@ def hip_fp8_prefill_attention(
     result is that call's over the dequantised pool. Arguments and errors as
     there; ``plan``: ``plan_fp8_prefill`` of this table and these lengths.
     """
+    out = None if plan is None else _prefill_native(plan, query, key, value, key_cache, value_cache,
+                                                    kv_scales, block_size)
+    if out is not None:
+        return out
     num_blocks, num_kv_heads, head_dim = _check_pool(key_cache, value_cache, kv_scales, block_size,
                                                      "hip_fp8_prefill_attention")
     total_q, num_q_heads, q_dim = query.shape
@@ -619,6 +676,11 @@ def hip_fp8_prefill_attention(
                     plan = plan_fp8_prefill(block_table, rows, cached, qlens, block_size, num_blocks,
                                             num_q_heads, num_kv_heads, head_dim, dtype, device)
                     _gpu._cache_put("fp8_prefill", (block_table,), extra, plan)
+                else:
+                    out = _prefill_native(plan, query, key, value, key_cache, value_cache, kv_scales,
+                                          block_size)
+                    if out is not None:
+                        return out
             assert plan.key == (block_size, num_blocks, num_q_heads, num_kv_heads, head_dim, dtype) and (
                 plan.device == device), "the plan is of another step or pool"
             total, made, n = plan.total, plan.plan, plan.num_seqs
@@ -715,7 +777,8 @@ def plan_fp8_gather(
                 f"block_table insufficient to cover the cached prefixes: {bad.item()} token(s) "
                 f"without a pool block"
             )
-        return Fp8GatherPlan(device, (slots,), _gpu._stream(device), total=total,
+        words = _hip.fp8_gather_words(slots.data_ptr(), total, block_size, num_blocks, device.index)
+        return Fp8GatherPlan(device, (slots,), _gpu._stream(device), words=words, total=total,
                              key=(block_size, num_blocks))
 
 
@@ -736,6 +799,16 @@ def gather_fp8_prefix_kv(
     bf16, the type the cache was written in), ``code * scale`` exactly. Errors as
     there; ``plan``: ``plan_fp8_gather`` of this table and these lengths.
     """
+    native = _hip.native_fp8
+    if plan is not None and native is not None and dtype in FP8_ROW_DTYPES:
+        stream = _gpu._stream(plan.device)
+        if stream == plan.stream:
+            out = native.gather(plan.words, key_cache, value_cache, kv_scales, block_size,
+                                dtype is torch.float16, stream)
+            if out is not None:
+                if type(out) is int:
+                    _hip.check(out, "mv_fp8_gather_kv")
+                return out
     num_blocks, num_kv_heads, head_dim = _check_pool(key_cache, value_cache, kv_scales, block_size,
                                                      "gather_fp8_prefix_kv")
     assert dtype in FP8_ROW_DTYPES, f"dtype {dtype} not supported (fp16, bf16)"

@@ -307,3 +307,47 @@ def test_backend_refusals():
             be.allocate_pool(1, 4, bs, 1, 64, dtype, DEV, cache_dtype=cache)
     pool = be.allocate_pool(1, 4, 16, 1, 64, torch.bfloat16, DEV, cache_dtype=torch.bfloat16)
     assert pool.kv_scales is None and pool.key_caches[0].dtype is torch.bfloat16
+
+
+@pytest.mark.parametrize("form", ["plan", "step"])
+def test_native_calls_equal_the_wrappers(form, monkeypatch):
+    """Three layers of a step through the native calls and with them off: the same
+    bits; what is not the plain case (strided K, another stream) is left to the
+    wrapper and gives them too."""
+    hq, hkv, d, bs, dtype, num_blocks = 14, 2, 64, 16, torch.bfloat16, 40
+    tables = torch.randperm(num_blocks, generator=torch.Generator().manual_seed(1))[:24].view(2, 12)
+    rope = _rope(d, dtype)
+    meta, slots, positions = _meta([(0, 20, 50), (1, 0, 9)], [], tables, bs)
+    bt, kv = tables.to(DEV), torch.tensor([70, 9], device=DEV)
+    rows, cached, new = [0, 1], [20, 0], [50, 9]
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(59, h, d, generator=g).to(dtype).to(DEV) for h in (hq, hkv, hkv))
+    odd = torch.empty(59, hkv, d + 4, dtype=dtype, device=DEV)[:, :, :d]
+    odd.copy_(k)  # (rows that are not 16-byte aligned)
+    results = []
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(fp8._hip, "native_fp8", None)
+        assert (fp8._hip.native_fp8 is not None) == native
+        kc, vc, sc = fp8_util.random_pool(num_blocks, hkv, bs, d, 1, DEV)
+        plans = [None] * 4
+        if form == "plan":
+            plans = [fp8.plan_fp8_write(slots, bs, num_blocks, DEV, positions, rope.cos.shape[0]),
+                     fp8.plan_fp8_decode(bt, kv, bs, num_blocks, DEV, d, hkv),
+                     fp8.plan_fp8_prefill(bt, rows, cached, new, bs, num_blocks, hq, hkv, d, dtype, DEV),
+                     fp8.plan_fp8_gather(bt, [70, 9], rows, bs, num_blocks, DEV)]
+        outs = []
+        for layer, (stream, key) in enumerate([(None, k), (None, k), (torch.cuda.Stream(), k), (None, odd)]):
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream) if stream else torch.cuda.stream(torch.cuda.current_stream()):
+                qr, kr = fp8.hip_fp8_rope_kv_cache_write(q, key, v, positions, rope.cos, rope.sin, kc, vc, sc,
+                                                         slots, bs, plan=plans[0])
+                outs += [qr, kr, fp8.hip_fp8_prefill_attention(qr, kr, v, kc, vc, sc, bt, rows, cached, new,
+                                                               bs, plan=plans[2])]
+                outs.append(fp8.hip_fp8_decode_attention(qr[:2], kc, vc, sc, bt, kv, bs, plan=plans[1]))
+                outs += fp8.gather_fp8_prefix_kv(kc, vc, sc, bt, [70, 9], rows, bs, dtype, plan=plans[3])
+            torch.cuda.synchronize()
+        results.append(outs)
+        gpu.invalidate_cached_metadata()
+    assert len(results[0]) == len(results[1]) == 24
+    assert all(torch.equal(bits(a), bits(b)) for a, b in zip(*results))
