@@ -717,11 +717,30 @@ int mv_fp8_kv_cache_write(
     int32_t block_size, int64_t num_blocks, int32_t dtype, void* stream);
 
 /*
- * Decode attention over the 8-bit pool: mv_paged_decode's arguments, the plan
- * made by mv_decode_plan with mv_fp8_decode_groups_per_cu; out rows 16-byte
- * aligned. V codes of places no sequence attends are not used.
+ * The plan of a decode step over the 8-bit pool: the work list, block ids,
+ * counters and status words of mv_decode_plan, cut into pieces by this kernel's
+ * own costs (joining pieces is dearer against its streaming). kv_len, block_table
+ * int32 or int64 (*_is_i64). fixed: a launch of fixed size (graph capture): every
+ * entry of work_items past the last group is marked unused, and the launch takes
+ * num_work_groups = work_capacity, partition_tokens and max_partitions from the
+ * bounds. mv_fp8_decode_plan_bounds writes, for any lengths, out[0] = work
+ * entries (8 ints each), out[1] = partition_tokens, out[2] = pieces of a
+ * sequence, out[3] = block ids (int32). counters: int32[num_seqs * num_kv_heads].
  */
-int mv_fp8_decode_groups_per_cu(int32_t head_dim);
+int mv_fp8_decode_plan_bounds(int32_t num_seqs, int32_t max_blocks, int32_t block_size,
+                              int32_t num_kv_heads, int32_t cu_count, int32_t fixed, int64_t* out);
+int mv_fp8_decode_plan(const void* kv_len, int32_t kv_len_is_i64, const void* block_table,
+                       int32_t bt_is_i64, int64_t bt_stride, int32_t num_seqs, int32_t max_blocks,
+                       int32_t block_size, int64_t num_blocks, int32_t num_kv_heads,
+                       int32_t head_dim, int32_t cu_count, int32_t fixed, int32_t* work_items,
+                       int64_t work_capacity, int32_t* block_ids, int64_t block_ids_capacity,
+                       int32_t* counters, int32_t* status, void* stream);
+
+/*
+ * Decode attention over the 8-bit pool: mv_paged_decode's arguments, with the
+ * plan of mv_fp8_decode_plan; out rows 16-byte aligned. V codes of places no
+ * sequence attends are not used.
+ */
 size_t mv_fp8_paged_decode_workspace_bytes(int32_t num_seqs, int32_t num_q_heads,
                                            int32_t head_dim, int32_t max_partitions);
 int mv_fp8_paged_decode(const void* query, int64_t q_stride_tok, int64_t q_stride_head,

@@ -3,8 +3,8 @@
 // p_j = exp(scale q k_j - m).
 //
 // Bound: HBM (14 flop per byte at 7 query heads per kv head), and on small
-// batches the chain of memory round trips. The work list is the decode plan's
-// (mv_decode_plan): one work group per (sequence, kv head, piece of its tokens).
+// batches the chain of memory round trips. The plan (fp8_decode_plan_kernel) gives
+// one work group per (sequence, kv head, piece of its tokens).
 //
 // The codes go from memory to registers to the matrix cores, without shared
 // memory, because both operand layouts can be loaded directly. A tile is 16
@@ -34,8 +34,10 @@
 namespace mv {
 namespace {
 
+constexpr int kDwPairs = 2;  // pairs of tiles in flight per wave
+constexpr int kRsrcWord3 = 0x00020000;  // raw buffer, 32-bit data
+constexpr int kStream = 2;              // non-temporal: every code is read once
 constexpr int kDwWaves = 4;
-constexpr int kDwThreads = kDwWaves * 64;
 constexpr float kDwFastMax = 4096.f;
 constexpr float kDwStart = -3e38f;  // the reference before a head's first token
 
@@ -75,13 +77,15 @@ struct TileCodes {
 };
 
 template <int DTYPE, int D>
-__global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a) {
+__global__ __launch_bounds__(kDwWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_decode_kernel(Fp8DecodeArgs a) {
+  constexpr int W = kDwWaves, P = kDwPairs;
   constexpr int KS = D / 32;  // MFMA steps of K Q^T
   constexpr int C = D / 16;   // MFMAs of V^T P^T
   constexpr int VW = D / 64;
   constexpr int kORow = D + 4;
-  __shared__ __attribute__((aligned(16))) float s_o[kDwWaves][16][kORow];
-  __shared__ float s_m[kDwWaves][16], s_l[kDwWaves][16];
+  constexpr int E = D / (4 * W);  // dims per thread of the merges: 4 W threads a head
+  __shared__ __attribute__((aligned(16))) float s_o[W][16][kORow];
+  __shared__ float s_m[W][16], s_l[W][16];
   __shared__ int s_last;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
   const int32_t* ids = a.block_ids + item * a.ids_per_item;
   const bool one = a.bs_log2 == 4;
   int id = 0;
-  if (one) id = ids[min(wave + kDwWaves * lane, a.ids_per_item - 1)];
+  if (one) id = ids[min(wave + W * lane, a.ids_per_item - 1)];
   const int4 w0 = reinterpret_cast<const int4*>(a.work + 8 * item)[0];
   const int4 w1 = reinterpret_cast<const int4*>(a.work + 8 * item)[1];
   if (w0.x < 0) return;  // an unused slot of a launch of fixed size
@@ -104,9 +108,9 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
   const int tok_begin = w1.x, tok_end = w1.y;
   const int first_blk = tok_begin >> a.bs_log2;
   const int tiles = (tok_end - tok_begin + kTile - 1) / kTile;
-  const int mine = (tiles - wave + kDwWaves - 1) / kDwWaves;  // this wave's tiles
+  const int mine = (tiles - wave + W - 1) / W;  // this wave's tiles
   auto id_of = [&](int j) {  // (lanes past the wave's tiles take its last one's)
-    const int tok = tok_begin + (wave + kDwWaves * min(j, mine - 1)) * kTile;
+    const int tok = tok_begin + (wave + W * min(j, mine - 1)) * kTile;
     return ids[min((tok >> a.bs_log2) - first_blk, a.ids_per_item - 1)];
   };
   if (!one && mine > 0) id = id_of(lane);
@@ -132,27 +136,32 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
     // an id outside the pool is never an address: its tiles read block 0 and
     // are masked
     const bool have = static_cast<uint32_t>(id) < a.num_blocks;
-    const int cur = have ? id : 0;
     const uint64_t have_mask = __builtin_amdgcn_ballot_w64(have);
-    const float2 s2 = reinterpret_cast<const float2*>(a.scales)[static_cast<int64_t>(cur) * a.num_kv_heads + h];
+    const int64_t bh = static_cast<int64_t>(have ? id : 0) * a.num_kv_heads + h;
+    const float2 s2 = reinterpret_cast<const float2*>(a.scales)[bh];
+    // this lane's tile's place in the pools, in bytes
+    const int my_tok = tok_begin + (wave + W * (j0 + lane)) * kTile;
+    const uint64_t at = static_cast<uint64_t>((bh << a.bs_log2) + (my_tok & ((1 << a.bs_log2) - 1))) * D;
+    const uint32_t at_lo = static_cast<uint32_t>(at), at_hi = static_cast<uint32_t>(at >> 32);
     if (j0 + 64 < mine) id = id_of(j0 + 64 + lane);
 
+    // (a buffer descriptor per tile: a tile past the window's last has no bytes,
+    // its loads return zeros without a memory access)
     auto load_tile = [&](int jw, TileCodes<D>& x) __attribute__((always_inline)) {
-      const int j = min(jw, nw - 1);
-      const int64_t blk = __builtin_amdgcn_readlane(cur, j);
-      const int tok = tok_begin + (wave + kDwWaves * (j0 + j)) * kTile;
-      const int64_t at = (((blk * a.num_kv_heads + h) << a.bs_log2) + (tok & ((1 << a.bs_log2) - 1))) * D;
-      const uint8_t* k = a.k_cache + at;
-      const uint8_t* v = a.v_cache + at;
+      const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(at_lo, jw & 63))) |
+                          static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(at_hi, jw & 63))) << 32;
+      const int bytes = jw < nw ? kTile * D : 0;
+      const auto k = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.k_cache) + at, 0, bytes, kRsrcWord3);
+      const auto v = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.v_cache) + at, 0, bytes, kRsrcWord3);
 #pragma unroll
       for (int i = 0; i < TileCodes<D>::KL; ++i)
-        x.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k + k_lane + 64 * i));
+        x.k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(k, k_lane + 64 * i, 0, kStream));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if constexpr (VW == 1) {
-          x.v[e][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(v + v_lane + 4 * e * D));
+          x.v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(v, v_lane + 4 * e * D, 0, kStream);
         } else {
-          const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(v + v_lane + 4 * e * D));
+          const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(v, v_lane + 4 * e * D, 0, kStream));
           x.v[e][0] = w[0];
           x.v[e][1] = w[1];
         }
@@ -186,17 +195,19 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
     };
     // Tiles jw and jw + 1 of the window.
     auto pair = [&](int jw, TileCodes<D>& xa, TileCodes<D>& xb) __attribute__((always_inline)) {
-      const int jb = min(jw + 1, 63);
-      const int tok_a = tok_begin + (wave + kDwWaves * (j0 + jw)) * kTile;
-      const int tok_b = tok_a + kDwWaves * kTile;
-      const int end_a = (have_mask >> jw) & 1 ? tok_end : 0;
-      const int end_b = jw + 1 < nw && ((have_mask >> jb) & 1) ? tok_end : 0;
+      // (jw is even: tile jw + 1 is in the window; past the wave's last one it
+      // lies past the piece's end)
+      const int jb = jw + 1;
+      const int tok_a = tok_begin + (wave + W * (j0 + jw)) * kTile;
+      const int tok_b = tok_a + W * kTile;
       const float ka = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s2.x), jw));
       const float kb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s2.x), jb));
       const float va = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s2.y), jw));
       const float vb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s2.y), jb));
       f32x4 sa = scores(xa, ka), sb = scores(xb, kb);
-      if (tok_a + kTile > end_a || tok_b + kTile > end_b) {
+      if (tok_b + kTile > tok_end || have_mask != ~uint64_t(0)) {
+        const int end_a = (have_mask >> jw) & 1 ? tok_end : 0;
+        const int end_b = (have_mask >> jb) & 1 ? tok_end : 0;
         // tokens that are not attended: score -inf, and V 0 (0 * NaN is NaN)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -246,25 +257,26 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
       for (int c = 0; c < C; ++c) o[c] = mfma16<DTYPE>(u32x4{oa[c][0], oa[c][1], ob[c][0], ob[c][1]}, p, o[c]);
     };
 
-    // Two pairs of tiles in flight: a pair is loaded while the one before it
-    // is computed. (Loads past the window's last tile repeat it.)
-    TileCodes<D> x[4];
+    // P pairs of tiles in flight: a pair's registers are loaded again as soon as it
+    // is computed.
+    TileCodes<D> x[2 * P];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_tile(i, x[i]);
+    for (int i = 0; i < 2 * P; ++i) load_tile(i, x[i]);
     int jw = 0;
-    for (; jw + 4 < nw; jw += 4) {
-      pair(jw, x[0], x[1]);
-      load_tile(jw + 4, x[0]);
-      load_tile(jw + 5, x[1]);
-      pair(jw + 2, x[2], x[3]);
-      load_tile(jw + 6, x[2]);
-      load_tile(jw + 7, x[3]);
+    for (; jw + 2 * P < nw; jw += 2 * P) {
+#pragma unroll
+      for (int i = 0; i < 2 * P; i += 2) {
+        pair(jw + i, x[i], x[i + 1]);
+        load_tile(jw + 2 * P + i, x[i]);
+        load_tile(jw + 2 * P + i + 1, x[i + 1]);
+      }
     }
-    pair(jw, x[0], x[1]);
-    if (jw + 2 < nw) pair(jw + 2, x[2], x[3]);
+#pragma unroll
+    for (int i = 0; i < 2 * P; i += 2)
+      if (jw + i < nw) pair(jw + i, x[i], x[i + 1]);
   }
 
-  // ---- merge the waves: thread (r, c) takes dims c D/16 .. of head r
+  // ---- merge the waves: thread (r, c) takes dims c E .. of head r
   l = rows_sum(l);
   if (!(l > 0.f)) m = kNegInf;  // saw no token (or NaN: kept in l)
   if (g == 0) {
@@ -278,41 +290,35 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
       *reinterpret_cast<float4*>(&s_o[wave][t][C * (4 * g + i) + x]) =
           make_float4(o[x][i], o[x + 1][i], o[x + 2][i], o[x + 3][i]);
   __syncthreads();
-  const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
+  const int r = threadIdx.x / (4 * W), c = threadIdx.x % (4 * W);
   const bool has_row = r < a.n_rep;
   float mx = kNegInf, sum = 0.f;
-  float v[C];
+  float v[E];
 #pragma unroll
-  for (int i = 0; i < C; ++i) v[i] = 0.f;
+  for (int i = 0; i < E; ++i) v[i] = 0.f;
 #pragma unroll
-  for (int w = 0; w < kDwWaves; ++w) mx = fmaxf(mx, s_m[w][r]);
+  for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w][r]);
 #pragma unroll
-  for (int w = 0; w < kDwWaves; ++w) {
+  for (int w = 0; w < W; ++w) {
     const float mw = s_m[w][r];
     const float f = mw == kNegInf ? (s_l[w][r] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mw - mx);
     sum += s_l[w][r] * f;
 #pragma unroll
-    for (int x = 0; x < C; x += 4) {
-      const float4 y = *reinterpret_cast<const float4*>(&s_o[w][r][C * c + x]);
+    for (int x = 0; x < E; x += 2) {
+      const float2 y = *reinterpret_cast<const float2*>(&s_o[w][r][E * c + x]);
       v[x] += y.x * f;
       v[x + 1] += y.y * f;
-      v[x + 2] += y.z * f;
-      v[x + 3] += y.w * f;
     }
   }
   const float inv = 1.f / sum;
 #pragma unroll
-  for (int i = 0; i < C; ++i) v[i] *= inv;
-  char* const dst = a.out + b * a.o_st + (h * a.n_rep + (has_row ? r : 0)) * a.o_sh + 2 * C * c;
-  auto store_row = [&](const float (&y)[C]) __attribute__((always_inline)) {
+  for (int i = 0; i < E; ++i) v[i] *= inv;
+  char* const dst = a.out + b * a.o_st + (h * a.n_rep + (has_row ? r : 0)) * a.o_sh + 2 * E * c;
+  auto store_row = [&](const float (&y)[E]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < C; x += 4) {
-      uint32_t w[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        w[i] = static_cast<uint32_t>(from_f32<DTYPE>(y[x + 2 * i])) | static_cast<uint32_t>(from_f32<DTYPE>(y[x + 2 * i + 1])) << 16;
-      *reinterpret_cast<uint2*>(dst + 2 * x) = make_uint2(w[0], w[1]);
-    }
+    for (int x = 0; x < E; x += 2)
+      *reinterpret_cast<uint32_t*>(dst + 2 * x) =
+          static_cast<uint32_t>(from_f32<DTYPE>(y[x])) | static_cast<uint32_t>(from_f32<DTYPE>(y[x + 1])) << 16;
   };
   if (n_parts == 1) {
     if (has_row) store_row(v);
@@ -324,9 +330,9 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
   // piece order, so the result does not depend on which one that is
   const int64_t slot0 = (static_cast<int64_t>(b) * a.num_q_heads + h * a.n_rep + (has_row ? r : 0)) * a.max_parts;
   if (has_row) {
-    uint64_t* po = reinterpret_cast<uint64_t*>(a.ws_o + (slot0 + part) * D + C * c);
+    uint64_t* po = reinterpret_cast<uint64_t*>(a.ws_o + (slot0 + part) * D + E * c);
 #pragma unroll
-    for (int x = 0; x < C; x += 2) store_coherent_u64(po + x / 2, pack_f32x2(v[x], v[x + 1]));
+    for (int x = 0; x < E; x += 2) store_coherent_u64(po + x / 2, pack_f32x2(v[x], v[x + 1]));
     if (c == 0) store_coherent_u64(reinterpret_cast<uint64_t*>(a.ws_ml) + slot0 + part, pack_f32x2(mx, sum));
   }
   asm volatile("" ::: "memory");
@@ -341,18 +347,18 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
   if (has_row) {
     float m_all = kNegInf, l_all = 0.f;
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = 0.f;
-    // rounds of 8 pieces, every load of a round in flight before the first use
-    constexpr int R = 512 / D;
+    for (int i = 0; i < E; ++i) v[i] = 0.f;
+    // rounds of 16 pieces, every load of a round in flight before the first use
+    constexpr int R = 16;
     for (int p0 = 0; p0 < n_parts; p0 += R) {
-      uint64_t ml[R], ov[R][C / 2];
+      uint64_t ml[R], ov[R][E / 2];
 #pragma unroll
       for (int p = 0; p < R; ++p) {
         const int64_t slot = slot0 + min(p0 + p, n_parts - 1);
         ml[p] = load_coherent_u64(reinterpret_cast<const uint64_t*>(a.ws_ml) + slot);
-        const uint64_t* src = reinterpret_cast<const uint64_t*>(a.ws_o + slot * D + C * c);
+        const uint64_t* src = reinterpret_cast<const uint64_t*>(a.ws_o + slot * D + E * c);
 #pragma unroll
-        for (int x = 0; x < C / 2; ++x) ov[p][x] = load_coherent_u64(src + x);
+        for (int x = 0; x < E / 2; ++x) ov[p][x] = load_coherent_u64(src + x);
       }
       float m_new = m_all;
 #pragma unroll
@@ -360,13 +366,13 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
       const float keep = m_all == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m_all - m_new);
       l_all *= keep;
 #pragma unroll
-      for (int i = 0; i < C; ++i) v[i] *= keep;
+      for (int i = 0; i < E; ++i) v[i] *= keep;
 #pragma unroll
       for (int p = 0; p < R; ++p) {
         const float w = p0 + p < n_parts ? unpack_hi(ml[p]) * __builtin_amdgcn_exp2f(unpack_lo(ml[p]) - m_new) : 0.f;
         l_all += w;
 #pragma unroll
-        for (int x = 0; x < C / 2; ++x) {
+        for (int x = 0; x < E / 2; ++x) {
           v[2 * x] += w * unpack_lo(ov[p][x]);
           v[2 * x + 1] += w * unpack_hi(ov[p][x]);
         }
@@ -375,11 +381,265 @@ __global__ __launch_bounds__(kDwThreads) void fp8_decode_kernel(Fp8DecodeArgs a)
     }
     const float inv_all = 1.f / l_all;
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] *= inv_all;
+    for (int i = 0; i < E; ++i) v[i] *= inv_all;
     store_row(v);
   }
   if (threadIdx.x == 0)  // ready for the next call
     __hip_atomic_store(&a.counters[b * a.num_kv_heads + h], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---------------------------------------------------------------- plan --
+//
+// Cuts each sequence's tokens into pieces of at most L tiles, one work group per
+// (sequence, kv head, piece), and deals the groups to the CUs. Joining pieces
+// costs a launch 2.4 us or more (three round trips to device-coherent memory), in
+// which one group streams 100 KB, so L is chosen by an estimate of the launch's
+// time; with C CUs, G groups and p pieces of a sequence in the mean, in us:
+//   all     = all bytes / the rate at which a full launch reads (6.3 TB/s)
+//   cu      = bytes of the busiest CU / the rate of one group (40 KB per us; 34 at
+//             head_dim 128, whose K rows are read in half lines)
+//   time(L) = (all^4 + cu^4)^(1/4) + (if any is cut: 2.4 + 0.18 (p - 1) G / C)
+//             + 0.4 (groups per CU - 1)
+// The busiest CU has the largest piece if there are at most C groups, that or
+// the mean plus a few percent for up to 3 C (all of them resident, dealt by
+// size), and what is left of the last rounds beyond. Fitted to 50 batches;
+// measured (us a call): 64 x 1024 tokens at 14 / 2 x 64 uncut 7.4, in 2 pieces
+// 8.5, in 4 9.2; 16 x 8k-32k one group per CU 19.8, two 21.6; 128 x 512-4096 at
+// 28 / 4 x 128 uncut, two groups per CU 52, cut for three 63.5; 256 x
+// lognormal(300) 11.3 cut for three, 25.8 uncut.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanDealt = 1024;    // groups of a launch that is dealt, at most
+constexpr int kPlanMaxParts = 128;  // pieces of a sequence
+constexpr int kPlanMinTiles = 4;    // tiles of a piece: one for each wave
+constexpr float kHbmBytesPerUs = 6.3e6f;
+constexpr float kMergeUs = 2.4f, kMergePartUs = 0.18f, kExtraGroupUs = 0.4f;
+
+// ids per work group: the blocks a piece may touch, to a multiple of 4
+__host__ __device__ inline int ids_stride(int64_t partition_tokens, int bs_log2) {
+  return static_cast<int>((((partition_tokens + (1 << bs_log2) - 1) >> bs_log2) + 1 + 3) & ~int64_t(3));
+}
+
+struct Fp8DecodePlanArgs {
+  const void* kv_len;
+  const void* block_table;
+  int64_t bt_stride, num_blocks;
+  int32_t num_seqs, max_blocks, bs_log2, num_kv_heads, cu_count, fixed;
+  int32_t kv_i64, bt_i64;
+  float cu_bytes_per_us, tile_bytes;
+  int32_t* work;
+  int64_t max_groups;  // of any plan of this batch
+  int64_t work_cap;    // entries of `work`
+  int32_t* block_ids;
+  int32_t* counters;
+  int32_t* status;
+};
+
+__device__ __forceinline__ int64_t int_at(const void* p, int i64, int64_t i) {
+  return i64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) x += __shfl_xor(x, s);
+  return x;
+}
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) x = max(x, __shfl_xor(x, s));
+  return x;
+}
+
+// Tiles of sequence b that are planned: 0 where its length is below 1 or past
+// its table row (reported).
+__device__ __forceinline__ int planned_tiles(const Fp8DecodePlanArgs& a, int64_t kv) {
+  if (kv < 1 || kv > (static_cast<int64_t>(a.max_blocks) << a.bs_log2)) return 0;
+  return static_cast<int>((kv + kTile - 1) / kTile);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void fp8_decode_plan_kernel(Fp8DecodePlanArgs a) {
+  __shared__ int s_a[kPlanWaves];
+  __shared__ float s_cost[kPlanWaves];
+  __shared__ int s_l[kPlanWaves];
+  __shared__ int s_bad, s_short, s_min, s_total, s_most, s_live, s_base;
+  __shared__ int s_size[kPlanDealt];
+  __shared__ int4 s_item[kPlanDealt];  // sequence, piece, pieces, kv head
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int H = a.num_kv_heads, C = a.cu_count;
+  if (tid == 0) {
+    s_bad = s_short = 0;
+    s_min = INT_MAX;
+    s_total = s_most = s_live = 0;
+    s_base = 0;
+  }
+  __syncthreads();
+  // ---- lengths: checks, all tiles, the most tiles of a sequence
+  {
+    int total = 0, most = 0, live = 0, bad = 0, over = 0, low = INT_MAX;
+    for (int b = tid; b < a.num_seqs; b += kPlanThreads) {
+      const int64_t kv = int_at(a.kv_len, a.kv_i64, b);
+      low = min(low, static_cast<int>(kv < INT_MIN ? INT_MIN : kv > INT_MAX ? INT_MAX : kv));
+      bad += kv < 1;
+      over += kv > (static_cast<int64_t>(a.max_blocks) << a.bs_log2);
+      const int t = planned_tiles(a, kv);
+      total += t;
+      live += t > 0;
+      most = max(most, t);
+    }
+    if (bad) atomicAdd(&s_bad, bad);
+    if (over) atomicAdd(&s_short, over);
+    atomicMin(&s_min, low);
+    atomicAdd(&s_total, total);
+    atomicAdd(&s_live, live);
+    atomicMax(&s_most, most);
+  }
+  for (int i = tid; i < a.num_seqs * H; i += kPlanThreads) a.counters[i] = 0;
+  __syncthreads();
+  const int total = s_total, most = s_most;
+  // ---- the piece bound L: every wave tries one, 16 over the whole range, then
+  // 16 around the best
+  int best = max(most, 1);
+  int groups = 0, parts = 1, longest = 1;
+  if (most > 0) {
+    const int least = min(most, max(kPlanMinTiles, (most + kPlanMaxParts - 1) / kPlanMaxParts));
+    int hi = most, lo = least;
+    for (int round = 0; round < 3; ++round) {
+      // round 2: the chosen L once more, for its groups, pieces and size
+      int L;
+      if (round == 0) L = static_cast<int>(most * exp2f(log2f(static_cast<float>(least) / most) * wave / (kPlanWaves - 1)) + 0.5f);
+      else if (round == 1) L = hi - static_cast<int>(static_cast<int64_t>(hi - lo) * wave / (kPlanWaves - 1));
+      else L = best;
+      L = min(max(L, least), most);
+      int n = 0, np_most = 1, piece = 1;
+      for (int b = lane; b < a.num_seqs; b += 64) {
+        const int t = planned_tiles(a, int_at(a.kv_len, a.kv_i64, b));
+        const int np = (t + L - 1) / L;
+        n += np;
+        np_most = max(np_most, np);
+        if (np > 0) piece = max(piece, (t + np - 1) / np);
+      }
+      n = wave_sum(n);
+      np_most = wave_max(np_most);
+      piece = wave_max(piece);
+      if (round == 2) {
+        groups = n * H;
+        parts = np_most;
+        longest = piece;
+        break;
+      }
+      const float G = static_cast<float>(n) * H, mean = static_cast<float>(total) * H / C;
+      float busiest = piece;
+      if (G > 3.f * C) busiest = mean * 1.1f + piece;
+      else if (G > C) busiest = fmaxf(busiest, mean * 1.05f);
+      const float all = static_cast<float>(total) * H * a.tile_bytes / kHbmBytesPerUs;
+      const float cu = busiest * a.tile_bytes / a.cu_bytes_per_us;
+      float cost = sqrtf(sqrtf(all * all * all * all + cu * cu * cu * cu)) +
+                   (np_most > 1 ? kMergeUs + kMergePartUs * (static_cast<float>(n) / s_live - 1.f) * G / C : 0.f) +
+                   kExtraGroupUs * fminf(ceilf(G / C) - 1.f, 3.f);
+      if (static_cast<int64_t>(n) * H > a.max_groups) cost = 3e38f;
+      if (lane == 0) {
+        s_cost[wave] = cost;
+        s_l[wave] = L;
+      }
+      __syncthreads();
+      int at = 0;
+      for (int w = 1; w < kPlanWaves; ++w)
+        if (s_cost[w] < s_cost[at]) at = w;  // (ties: the larger L)
+      best = s_l[at];
+      hi = s_l[max(at - 1, 0)];
+      lo = s_l[min(at + 1, kPlanWaves - 1)];
+      __syncthreads();
+    }
+  }
+  // ---- the groups, in sequence order; up to 3 C of them (and what LDS holds)
+  // are dealt: by size, largest first, in snake order over the CUs, on which
+  // group i and group i + C run
+  const bool dealt = groups <= min(3 * C, kPlanDealt);
+  for (int b0 = 0; b0 < a.num_seqs; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int64_t kv = b < a.num_seqs ? int_at(a.kv_len, a.kv_i64, b) : 0;
+    const int t = b < a.num_seqs ? planned_tiles(a, kv) : 0;
+    const int np = (t + best - 1) / best;
+    int incl = np;  // pieces up to and with sequence b
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int y = __shfl_up(incl, s);
+      if (lane >= s) incl += y;
+    }
+    if (lane == 63) s_a[wave] = incl;
+    __syncthreads();
+    int before = s_base;
+    for (int w = 0; w < wave; ++w) before += s_a[w];
+    const int first = before + incl - np;
+    for (int j = 0; j < np; ++j) {
+      const int q = t / np, r = t - q * np;
+      for (int h = 0; h < H; ++h) {
+        const int i = (first + j) * H + h;
+        if (dealt) {
+          s_size[i] = q + (j < r);
+          s_item[i] = make_int4(b, j, np, h);
+        } else {
+          const int start = j * q + min(j, r);
+          int4* e = reinterpret_cast<int4*>(a.work) + 2 * static_cast<int64_t>(i);
+          e[0] = make_int4(b, h, j, np);
+          e[1] = make_int4(start * kTile, static_cast<int>(min(kv, static_cast<int64_t>(start + q + (j < r)) * kTile)), 0, 0);
+        }
+      }
+    }
+    __syncthreads();
+    if (tid == kPlanThreads - 1) s_base = before + incl;
+    __syncthreads();
+  }
+  if (dealt && tid < groups) {
+    const int mine = s_size[tid];
+    int rank = 0;
+    for (int i = 0; i < groups; ++i) rank += s_size[i] > mine || (s_size[i] == mine && i < tid);
+    const int round = rank / C, pos = rank - round * C;
+    const int in_round = min(C, groups - round * C);
+    const int slot = round * C + ((round & 1) ? in_round - 1 - pos : pos);
+    const int4 it = s_item[tid];
+    const int64_t kv = int_at(a.kv_len, a.kv_i64, it.x);
+    const int t = planned_tiles(a, kv), q = t / it.z, r = t - q * it.z;
+    const int start = it.y * q + min(it.y, r);
+    int4* e = reinterpret_cast<int4*>(a.work) + 2 * static_cast<int64_t>(slot);
+    e[0] = make_int4(it.x, it.w, it.y, it.z);
+    e[1] = make_int4(start * kTile, static_cast<int>(min(kv, static_cast<int64_t>(start + mine) * kTile)), 0, 0);
+  }
+  if (a.fixed)
+    for (int64_t i = groups + tid; i < a.work_cap; i += kPlanThreads)
+      reinterpret_cast<int4*>(a.work)[2 * i] = make_int4(-1, 0, 0, 0);
+  if (tid == 0) {
+    a.status[MV_PLAN_NUM_ITEMS] = groups;
+    a.status[MV_PLAN_BAD_KV_LEN] = s_bad;
+    a.status[MV_PLAN_INSUFFICIENT] = s_short;
+    a.status[MV_PLAN_BAD_BLOCK] = 0;
+    a.status[MV_PLAN_MAX_PARTS] = parts;
+    a.status[MV_PLAN_MIN_KV_LEN] = s_min;
+    a.status[MV_PLAN_PARTITION_TOKENS] = longest * kTile;
+    a.status[MV_PLAN_IDS_PER_ITEM] =
+        ids_stride(a.fixed ? static_cast<int64_t>(a.max_blocks) << a.bs_log2 : static_cast<int64_t>(longest) * kTile, a.bs_log2);
+  }
+}
+
+// The pool blocks of every group's piece, a wave per group; an entry that is
+// not a pool block becomes -1 (its tokens are masked) and is counted once, by kv
+// head 0's piece that holds its first token.
+__global__ __launch_bounds__(256) void fp8_decode_ids_kernel(Fp8DecodePlanArgs a) {
+  const int64_t slot = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (slot >= a.status[MV_PLAN_NUM_ITEMS]) return;
+  const int4 e0 = reinterpret_cast<const int4*>(a.work)[2 * slot], e1 = reinterpret_cast<const int4*>(a.work)[2 * slot + 1];
+  const int first = e1.x >> a.bs_log2, n = ((e1.y - 1) >> a.bs_log2) - first + 1;
+  int32_t* ids = a.block_ids + slot * a.status[MV_PLAN_IDS_PER_ITEM];
+  int bad = 0;
+  for (int i = lane; i < n; i += 64) {
+    const int64_t blk = int_at(a.block_table, a.bt_i64, e0.x * a.bt_stride + first + i);
+    const bool ok = blk >= 0 && blk < a.num_blocks;
+    ids[i] = ok ? static_cast<int32_t>(blk) : -1;
+    bad += !ok && e0.y == 0 && ((first + i) << a.bs_log2) >= e1.x;
+  }
+  bad = wave_sum(bad);
+  if (bad && lane == 0) atomicAdd(&a.status[MV_PLAN_BAD_BLOCK], bad);
 }
 
 size_t ws_rows_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t head_dim, int32_t max_parts) {
@@ -387,16 +647,82 @@ size_t ws_rows_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t head_dim, in
   return (n + 255) / 256 * 256;
 }
 
-// ids per work group, as mv_decode_plan lays the lists out
-int ids_stride(int partition_tokens, int bs_log2) {
-  return (((partition_tokens + (1 << bs_log2) - 1) >> bs_log2) + 1 + 3) & ~3;
-}
-
 }  // namespace
 }  // namespace mv
 
-extern "C" int mv_fp8_decode_groups_per_cu(int32_t head_dim) {
-  return head_dim == 64 || head_dim == 128 ? 3 : 0;
+extern "C" int mv_fp8_decode_plan_bounds(int32_t num_seqs, int32_t max_blocks, int32_t block_size,
+                                         int32_t num_kv_heads, int32_t cu_count, int32_t fixed, int64_t* out) {
+  using namespace mv;
+  if (!out) return fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_decode_plan_bounds: null out");
+  if (num_seqs < 0 || max_blocks < 0 || num_kv_heads <= 0 || cu_count <= 0)
+    return fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_decode_plan_bounds: bad sizes");
+  if (!is_pow2(block_size) || block_size < 16 || block_size > 256)
+    return fail(MV_ERR_UNSUPPORTED, "mv_fp8_decode_plan_bounds: block_size %d (a power of two from 16 to 256)", block_size);
+  const int64_t units = static_cast<int64_t>(num_seqs) * num_kv_heads;
+  const int64_t tokens = static_cast<int64_t>(max_blocks) * block_size;
+  const int64_t tiles = (tokens + kTile - 1) / kTile;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kPlanMaxParts, (tiles + kPlanMinTiles - 1) / kPlanMinTiles));
+  const int64_t groups = std::min(units * parts, units + 3 * static_cast<int64_t>(cu_count));
+  if (tokens > INT_MAX / 2 || groups > INT_MAX / 8 || static_cast<int64_t>(num_seqs) * tiles > INT_MAX)
+    return fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_decode_plan_bounds: batch too large");
+  // ids: a launch of fixed size strides its lists by the whole table row; else
+  // by pieces of L tiles, at most units + all tiles / L of them:
+  // (units + units max_blocks bs / (16 L)) (16 L / bs + 8) with 16 L <= max_blocks bs
+  const int64_t ids = fixed ? groups * ids_stride(tokens, ilog2_exact(block_size))
+                            : 2 * units * max_blocks + 8 * (units + groups);
+  out[0] = groups;
+  out[1] = tokens;
+  out[2] = parts;
+  out[3] = ids;
+  return MV_OK;
+}
+
+extern "C" int mv_fp8_decode_plan(const void* kv_len, int32_t kv_len_is_i64, const void* block_table,
+                                  int32_t bt_is_i64, int64_t bt_stride, int32_t num_seqs, int32_t max_blocks,
+                                  int32_t block_size, int64_t num_blocks, int32_t num_kv_heads, int32_t head_dim,
+                                  int32_t cu_count, int32_t fixed, int32_t* work_items, int64_t work_capacity,
+                                  int32_t* block_ids, int64_t block_ids_capacity, int32_t* counters, int32_t* status,
+                                  void* stream) {
+  using namespace mv;
+  int64_t need[4];
+  const int rc = mv_fp8_decode_plan_bounds(num_seqs, max_blocks, block_size, num_kv_heads, cu_count, fixed, need);
+  if (rc != MV_OK) return rc;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(MV_ERR_UNSUPPORTED, "mv_fp8_decode_plan: head_dim %d not supported (64, 128)", head_dim);
+  if (!status || (num_seqs > 0 && (!kv_len || !counters || !work_items || !block_ids || (max_blocks > 0 && !block_table))))
+    return fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_decode_plan: null pointer");
+  if (num_blocks <= 0 || num_blocks > INT_MAX || work_capacity < need[0] || block_ids_capacity < need[3])
+    return fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_decode_plan: %lld blocks, capacities %lld and %lld (need %lld and %lld)",
+                static_cast<long long>(num_blocks), static_cast<long long>(work_capacity),
+                static_cast<long long>(block_ids_capacity), static_cast<long long>(need[0]),
+                static_cast<long long>(need[3]));
+  if (reinterpret_cast<uintptr_t>(work_items) % 16)
+    return fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_decode_plan: work list not 16-byte aligned");
+  Fp8DecodePlanArgs a;
+  a.kv_len = kv_len;
+  a.block_table = block_table;
+  a.bt_stride = bt_stride;
+  a.num_blocks = num_blocks;
+  a.num_seqs = num_seqs;
+  a.max_blocks = max_blocks;
+  a.bs_log2 = ilog2_exact(block_size);
+  a.num_kv_heads = num_kv_heads;
+  a.cu_count = cu_count;
+  a.fixed = fixed;
+  a.kv_i64 = kv_len_is_i64 != 0;
+  a.bt_i64 = bt_is_i64 != 0;
+  a.cu_bytes_per_us = head_dim == 64 ? 40e3f : 34e3f;
+  a.tile_bytes = 2.f * kTile * head_dim;
+  a.work = work_items;
+  a.max_groups = need[0];
+  a.work_cap = work_capacity;
+  a.block_ids = block_ids;
+  a.counters = counters;
+  a.status = status;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  fp8_decode_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+  if (need[0] > 0) fp8_decode_ids_kernel<<<static_cast<unsigned>((need[0] + 3) / 4), 256, 0, s>>>(a);
+  return check_launch("mv_fp8_decode_plan");
 }
 
 extern "C" size_t mv_fp8_paged_decode_workspace_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t head_dim,
@@ -479,11 +805,11 @@ extern "C" int mv_fp8_paged_decode(const void* query, int64_t q_stride_tok, int6
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(num_work_groups);
   if (dtype == MV_DTYPE_F16) {
-    if (head_dim == 64) fp8_decode_kernel<MV_DTYPE_F16, 64><<<grid, kDwThreads, 0, s>>>(a);
-    else fp8_decode_kernel<MV_DTYPE_F16, 128><<<grid, kDwThreads, 0, s>>>(a);
+    if (head_dim == 64) fp8_decode_kernel<MV_DTYPE_F16, 64><<<grid, kDwWaves * 64, 0, s>>>(a);
+    else fp8_decode_kernel<MV_DTYPE_F16, 128><<<grid, kDwWaves * 64, 0, s>>>(a);
   } else {
-    if (head_dim == 64) fp8_decode_kernel<MV_DTYPE_BF16, 64><<<grid, kDwThreads, 0, s>>>(a);
-    else fp8_decode_kernel<MV_DTYPE_BF16, 128><<<grid, kDwThreads, 0, s>>>(a);
+    if (head_dim == 64) fp8_decode_kernel<MV_DTYPE_BF16, 64><<<grid, kDwWaves * 64, 0, s>>>(a);
+    else fp8_decode_kernel<MV_DTYPE_BF16, 128><<<grid, kDwWaves * 64, 0, s>>>(a);
   }
   return check_launch("mv_fp8_paged_decode");
 }

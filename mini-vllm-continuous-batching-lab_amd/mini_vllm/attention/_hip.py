@@ -239,7 +239,14 @@ SIGNATURES = {
         _I64, _I32, _I32, _I32,    # num_tokens, num_q_heads, num_kv_heads, head_dim
         _I32, _I64, _I32, _P,      # block_size, num_blocks, dtype, stream
     ]),
-    "mv_fp8_decode_groups_per_cu": (ctypes.c_int, [_I32]),
+    "mv_fp8_decode_plan_bounds": (ctypes.c_int, [_I32, _I32, _I32, _I32, _I32, _I32, _P]),
+    "mv_fp8_decode_plan": (ctypes.c_int, [
+        _P, _I32, _P, _I32, _I64,  # kv_len, is_i64, block_table, is_i64, bt_stride
+        _I32, _I32, _I32, _I64,    # num_seqs, max_blocks, block_size, num_blocks
+        _I32, _I32, _I32, _I32,    # num_kv_heads, head_dim, cu_count, fixed
+        _P, _I64, _P, _I64,        # work_items, capacity, block_ids, capacity
+        _P, _P, _P,                # counters, status, stream
+    ]),
     "mv_fp8_paged_decode_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
     "mv_fp8_paged_decode": (ctypes.c_int, [
         _P, _I64, _I64,            # query, strides

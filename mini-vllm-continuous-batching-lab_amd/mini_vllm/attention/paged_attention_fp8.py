@@ -38,6 +38,7 @@ graph, a call without a plan records the planning too, and its checks raise from
 from __future__ import annotations
 
 import contextlib
+import ctypes
 from dataclasses import dataclass, field
 from typing import Optional, Sequence, Tuple
 
@@ -414,8 +415,8 @@ def hip_fp8_rope_kv_cache_write(
 
 @dataclass
 class Fp8DecodePlan(_Plan):
-    """A decode step's work list (``mv_decode_plan``) and its merge workspaces
-    per query-head count."""
+    """A decode step's work list (``mv_fp8_decode_plan``) and its merge
+    workspaces per query-head count."""
 
     plan: _gpu.DecodePlan = None
     key: tuple = ()  # (num_seqs, block_size, num_blocks, head_dim, num_kv_heads)
@@ -441,30 +442,75 @@ def plan_fp8_decode(
     head_dim: int,
     num_kv_heads: int,
 ) -> Fp8DecodePlan:
-    """``plan_decode`` for an 8-bit pool, with the same errors: ``ValueError``
-    for lengths below 1, ``IndexError`` for tables that do not cover them."""
+    """The work list of a decode step over an 8-bit pool, with ``plan_decode``'s
+    errors: ``ValueError`` for lengths below 1, ``IndexError`` for tables that do
+    not cover them or hold something else than pool blocks."""
     device = _indexed(torch.device(device))
     assert block_size in FP8_BLOCK_SIZES, (
         f"block_size {block_size} not supported (a power of 2 from 16 to 256)"
     )
     assert head_dim in _gpu.SUPPORTED_HEAD_DIMS, f"head_dim {head_dim} not supported (only 64, 128)"
     assert block_table.dim() == 2 and block_table.shape[0] == kv_len_after.shape[0]
+    lib = _hip.load()
     with _on(device):
         capture = _gpu._capture_id(device)
-        split = _gpu._groups_per_cu(device, head_dim, FP8_DTYPE)
-        pending = _gpu._plan_launch(block_table, kv_len_after, block_size, num_blocks, device,
-                                    head_dim, FP8_DTYPE, num_kv_heads, split, capture)
-        if pending.fixed:
-            _gpu._defer(capture, pending.raise_plan, pending.status)
-            made = _gpu._plan_finish(pending, None)
-        elif capture:
-            raise IndexError("block_table with 0 blocks per row is insufficient to cover kv_len_after")
+        bt, kv = _gpu._decode_metadata(block_table, kv_len_after, device)
+        num_seqs, max_blocks = bt.shape
+        cus = torch.cuda.get_device_properties(device).multi_processor_count
+        bounds = (ctypes.c_int64 * 4)()
+        _hip.check(lib.mv_fp8_decode_plan_bounds(num_seqs, max_blocks, block_size, num_kv_heads, cus,
+                                                 int(bool(capture)), bounds),
+                   "mv_fp8_decode_plan_bounds")
+        cap, most_tokens, most_parts, n_ids = bounds
+        # work list, block ids, counters and status words in one buffer, each part
+        # 16-byte aligned
+        n_work, n_ids = 8 * max(cap, 1), -(-max(n_ids, 4) // 4) * 4
+        n_units = max(num_seqs * num_kv_heads, 1)
+        n_cnt = -(-n_units // 4) * 4
+        buf = torch.empty(n_work + n_ids + n_cnt + _hip.MV_PLAN_WORDS, dtype=torch.int32, device=device)
+        base = buf.data_ptr()
+        _hip.check(
+            lib.mv_fp8_decode_plan(
+                _gpu._ptr(kv), int(kv.dtype == torch.int64), bt.data_ptr() if bt.numel() else None,
+                int(bt.dtype == torch.int64), bt.stride(0), num_seqs, max_blocks, block_size,
+                num_blocks, num_kv_heads, head_dim, cus, int(bool(capture)), base, cap,
+                base + 4 * n_work, n_ids, base + 4 * (n_work + n_ids),
+                base + 4 * (n_work + n_ids + n_cnt), _gpu._stream(device),
+            ),
+            "mv_fp8_decode_plan",
+        )
+        status = buf[n_work + n_ids + n_cnt:]
+
+        def raise_plan(st) -> None:
+            if st[_hip.MV_PLAN_BAD_KV_LEN]:
+                raise ValueError(
+                    f"kv_len_after must be >= 1 for all decode sequences, "
+                    f"got min={st[_hip.MV_PLAN_MIN_KV_LEN]}"
+                )
+            if st[_hip.MV_PLAN_INSUFFICIENT]:
+                raise IndexError(
+                    f"block_table with {max_blocks} blocks per row (block_size={block_size}) is "
+                    f"insufficient to cover kv_len_after for {st[_hip.MV_PLAN_INSUFFICIENT]} "
+                    f"sequence(s)"
+                )
+            if st[_hip.MV_PLAN_BAD_BLOCK]:
+                raise IndexError(
+                    f"block_table has {st[_hip.MV_PLAN_BAD_BLOCK]} entr(ies) within kv_len_after "
+                    f"that are not pool blocks [0, {num_blocks})"
+                )
+
+        if capture:
+            _gpu._defer(capture, raise_plan, status)
+            groups, parts, tokens = cap, most_parts, most_tokens
         else:
-            made = _gpu._plan_finish(pending, pending.status.tolist())
-        return Fp8DecodePlan(device, (made.work, made.block_ids, made.counters),
-                             _gpu._stream(device), capture, plan=made,
-                             key=(kv_len_after.shape[0], block_size, num_blocks, head_dim,
-                                  num_kv_heads))
+            st = status.tolist()
+            raise_plan(st)
+            groups, parts, tokens = (st[_hip.MV_PLAN_NUM_ITEMS], st[_hip.MV_PLAN_MAX_PARTS],
+                                     st[_hip.MV_PLAN_PARTITION_TOKENS])
+        made = _gpu.DecodePlan(buf[:n_work], buf[n_work:n_work + n_ids],
+                               buf[n_work + n_ids:n_work + n_ids + n_units], groups, parts, tokens)
+        return Fp8DecodePlan(device, (buf,), _gpu._stream(device), capture, plan=made,
+                             key=(num_seqs, block_size, num_blocks, head_dim, num_kv_heads))
 
 
 def hip_fp8_decode_attention(

@@ -484,9 +484,7 @@ def _groups_per_cu(device: torch.device, head_dim: int, dtype: torch.dtype) -> T
     if split is None:
         cus = torch.cuda.get_device_properties(device).multi_processor_count
         per_cu = os.environ.get("MVATTN_GROUPS_PER_CU")
-        if per_cu is None and dtype is torch.float8_e4m3fn:
-            per_cu = _hip.load().mv_fp8_decode_groups_per_cu(head_dim)
-        elif per_cu is None:
+        if per_cu is None:
             per_cu = _hip.load().mv_decode_groups_per_cu(head_dim, _hip.MV_DTYPE[dtype])
         split = _SPLIT[key] = (max(1, int(per_cu)), cus)
     return split

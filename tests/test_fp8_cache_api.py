@@ -33,6 +33,8 @@ WRITE = dict(q=BUF, q_st=64, q_sh=64, qo=BUF, qo_st=64, qo_sh=64, k=BUF, k_st=64
              ko_st=64, ko_sh=64, v=BUF, v_st=64, v_sh=64, kc=BUF, vc=BUF, scales=BUF, items=BUF,
              table=BUF, status=BUF, max_items=4, pos=BUF, cos=BUF, sin=BUF, table_st=64, max_pos=10,
              n=4, hq=2, hkv=1, d=64, bs=16, nb=8, dtype=2, stream=None)
+DPLAN = dict(kv=BUF, kv64=1, bt=BUF, bt64=1, bt_st=4, n=2, width=4, bs=16, nb=8, hkv=1, d=64, cus=256,
+             fixed=0, work=BUF, cap=512, ids=BUF, ids_cap=8192, counters=BUF, status=BUF, stream=None)
 DECODE = dict(q=BUF, q_st=64, q_sh=64, kc=BUF, vc=BUF, scales=BUF, work=BUF, ids=BUF, ids_cap=64,
               groups=1, part=16, parts=1, counters=BUF, out=BUF, o_st=64, o_sh=64, scale=0.125, b=1,
               hq=2, hkv=1, d=64, bs=16, nb=8, dtype=2, ws=None, ws_bytes=0, stream=None)
@@ -45,7 +47,7 @@ SLOTS = dict(bt=BUF, i64=1, bt_st=4, rows=1, width=4, seq_rows=BUF, cu=BUF, n=1,
 GATHER = dict(kc=BUF, vc=BUF, scales=BUF, slots=BUF, total=4, ok=BUF, ov=BUF, hkv=1, d=64, bs=16,
               nb=8, dtype=2, stream=None)
 ENTRIES = {
-    "mv_fp8_write_plan": PLAN, "mv_fp8_kv_cache_write": WRITE, "mv_fp8_paged_decode": DECODE,
+    "mv_fp8_decode_plan": DPLAN, "mv_fp8_write_plan": PLAN, "mv_fp8_kv_cache_write": WRITE, "mv_fp8_paged_decode": DECODE,
     "mv_fp8_paged_prefill": PREFILL, "mv_fp8_prefix_slots": SLOTS, "mv_fp8_gather_kv": GATHER,
 }
 INVALID, UNSUPPORTED = _hip.MV_ERR_INVALID_ARGUMENT, _hip.MV_ERR_UNSUPPORTED
@@ -66,6 +68,13 @@ REFUSED = [
     ("mv_fp8_kv_cache_write", dict(cos=None), INVALID),  # a query without tables
     ("mv_fp8_kv_cache_write", dict(k=BUF + 2), INVALID), ("mv_fp8_kv_cache_write", dict(v_st=65), INVALID),
     ("mv_fp8_kv_cache_write", dict(table_st=65), INVALID),
+    ("mv_fp8_decode_plan", dict(bs=8), UNSUPPORTED), ("mv_fp8_decode_plan", dict(d=96), UNSUPPORTED),
+    ("mv_fp8_decode_plan", dict(n=-1), INVALID), ("mv_fp8_decode_plan", dict(hkv=0), INVALID),
+    ("mv_fp8_decode_plan", dict(cus=0), INVALID), ("mv_fp8_decode_plan", dict(nb=0), INVALID),
+    ("mv_fp8_decode_plan", dict(cap=1), INVALID), ("mv_fp8_decode_plan", dict(ids_cap=16), INVALID),
+    ("mv_fp8_decode_plan", dict(status=None), INVALID), ("mv_fp8_decode_plan", dict(kv=None), INVALID),
+    ("mv_fp8_decode_plan", dict(bt=None), INVALID), ("mv_fp8_decode_plan", dict(work=BUF + 4), INVALID),
+    ("mv_fp8_decode_plan", dict(width=1 << 30), INVALID),
     ("mv_fp8_paged_decode", dict(dtype=0), UNSUPPORTED), ("mv_fp8_paged_decode", dict(d=32), UNSUPPORTED),
     ("mv_fp8_paged_decode", dict(bs=4), UNSUPPORTED), ("mv_fp8_paged_decode", dict(hq=17), UNSUPPORTED),
     ("mv_fp8_paged_decode", dict(hq=3, hkv=2), INVALID), ("mv_fp8_paged_decode", dict(scales=None), INVALID),
