@@ -45,7 +45,7 @@ constexpr float kPfStart = -3e38f;
 
 // RW row waves of 32 query rows x SETS key sets that split every stage's
 // tiles; a stage holds T tiles of 32 keys for each set, two stages in LDS. FP8:
-// the pool holds 8-bit codes (Fp8SubTileCopy).
+// the pool holds 8-bit codes (Fp8SubTile).
 template <int DTYPE_, int D_, int RW_, int SETS_, bool FP8_ = false>
 struct Prefill16Traits : TileGeom<DTYPE_, D_> {
   using G = TileGeom<DTYPE_, D_>;
@@ -93,27 +93,73 @@ __device__ __forceinline__ float halves_sum(float x) {
 
 // The K/V copies over a pool of 8-bit codes. A sub-tile of 16 prefix keys lies
 // in one pool block (of 16 tokens or more), so it has one K and one V scale. Its
-// codes are copied to LDS as they are, to the first half of their tile, and
-// turned into the tile's 16-bit values in place when the stage lands: the
+// codes become the tile's 16-bit values in LDS when the stage lands: the
 // conversion is done once per work group, not by every wave that reads the tile,
-// holds no registers while the copies are in flight (at head_dim 128 there are
-// none left), and what follows is the kernel of a 16-bit pool. Chunk keys are
-// copied as there. Of the one sub-tile across the prefix's end the codes go to
-// an LDS area of their own, and then to the prefix's rows. HALF: a wave
-// copies K (v false) or V only.
+// and what follows is the kernel of a 16-bit pool. Until then the codes are held
+// in registers (kRegs), loaded a whole stage ahead; where a wave copies K and V at
+// head_dim 128 there are none left, and they are copied to LDS as they are, to
+// the first half of their tile (those of the one sub-tile across the prefix's end
+// to an area of their own), and converted in place. Chunk keys are copied as in
+// the kernel of a 16-bit pool. HALF: a wave copies K (v false) or V only. Measured
+// (us, 4 x (1536 + 512) at 14 / 2 x 64; 8 x (300-2900 + 100-900) at 28 / 4 x 128):
+// all in place 30.6 and 133; as it is 29.3 and 125, where a 16-bit pool takes
+// 24.5 and 116. Without the conversion and its LDS stores it is 27.5 and 117.
 template <int DTYPE, int D, bool HALF>
 struct Fp8SubTile {
   using B = SubTileCopy<DTYPE, D>;
   static constexpr int CL = D / 64, NT = HALF ? 1 : 2;
   static constexpr int kCodeBytes = kTile * D;
+  static constexpr bool kRegs = D == 64 || HALF;
+  u32x4 codes[kRegs ? NT : 1][kRegs ? CL : 1];
   float scale[NT];
   int rows;  // prefix rows of the sub-tile in flight
 
-  // Starts the copies of keys kb .. kb + 15 to LDS address dst; returns the loads
-  // of the 16-bit copy whose rows are not to be cleared.
-  __device__ __forceinline__ unsigned fetch(const B& copy, int kb, int win_blk0, uint32_t dst, uint32_t mix,
-                                            int block_id, bool v) {
+  // Starts the loads of the codes of the sub-tile that begins with key kb; their
+  // LDS address dst and the mixed sub-tile's are of no use with kRegs.
+  __device__ __forceinline__ void fetch(const B& copy, int kb, uint32_t dst, uint32_t mix, int block_id, bool v) {
     rows = min(max(copy.cached - kb, 0), kTile);
+    if (rows == 0) return;
+    const PrefillArgs& a = copy.a;
+    const uint32_t code_dst = rows < kTile ? mix : dst;
+    const int code_step = rows < kTile ? kCodeBytes : B::G::kTileBytes;
+    const int id = __builtin_amdgcn_readfirstlane(block_id);
+    const bool ok = static_cast<uint32_t>(id) < a.num_blocks_u32;
+    const int64_t bh = (ok ? static_cast<int64_t>(id) : 0) * a.num_kv_heads + copy.h;
+    const int64_t at = ((bh << a.bs_log2) + (kb & ((1 << a.bs_log2) - 1))) * D;
+    // lane l of load c: row l / 4, 16 dims from 64 c + 16 (l % 4) (the 16-bit rows'
+    // stores then fall into different banks)
+    int lane = copy.lane;
+    asm volatile("" : "+v"(lane));
+    const uint32_t lane_off = (lane >> 2) * D + (lane & 3) * 16;
+    // (vector loads of the scales: a scalar load in flight would turn every LDS
+    // wait until its use into one for it)
+    const float* scales = a.kv_scales + 2 * bh + (lane >> 6);
+    if constexpr (HALF) {
+      scale[0] = scales[v ? 1 : 0];
+    } else {
+      const float2 s2 = *reinterpret_cast<const float2*>(scales);
+      scale[0] = s2.x;
+      scale[1] = s2.y;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool is_v = HALF ? v : n == 1;
+      const char* src = (is_v ? a.v_cache : a.k_cache) + at;
+#pragma unroll
+      for (int c = 0; c < CL; ++c) {
+        if constexpr (kRegs)
+          codes[n][c] = *reinterpret_cast<const u32x4*>(src + c * 64 + lane_off);
+        else
+          copy_to_lds_16B_sv(src + c * 64, lane_off,
+                             __builtin_amdgcn_readfirstlane(code_dst + (is_v ? code_step : 0) + c * 1024));
+      }
+    }
+  }
+
+  // Starts the 16-bit copies of the same sub-tile's chunk keys to LDS address dst;
+  // returns the loads of which no row is to be cleared.
+  __device__ __forceinline__ unsigned copy_rows(const B& copy, int kb, int win_blk0, uint32_t dst, int block_id,
+                                                bool v) const {
     if (rows == 0) {
       if constexpr (HALF) {
         if (v) return copy.template copy<false, true>(kb, win_blk0, dst, block_id);
@@ -123,73 +169,50 @@ struct Fp8SubTile {
         return copy.copy(kb, win_blk0, dst, block_id);
       }
     }
+    if (rows == kTile) return B::kAllValid;
     const PrefillArgs& a = copy.a;
-    unsigned valid = B::kAllValid;
-    uint32_t code_dst = dst;
-    int code_step = B::G::kTileBytes;
-    if (rows < kTile) {
-      code_dst = mix;
-      code_step = kCodeBytes;
-      valid = 0;
-      int lane_l = copy.lane;
-      asm volatile("" : "+v"(lane_l));  // (as in the 16-bit copy)
+    unsigned valid = 0;
+    int lane_l = copy.lane;
+    asm volatile("" : "+v"(lane_l));  // (as in the 16-bit copy)
 #pragma unroll
-      for (int c = 0; c < B::L; ++c) {
-        const int j = kb + B::row_of(lane_l, c);
-        const bool ok = j >= copy.cached && j < copy.key_end;
-        const int64_t cr = copy.chunk_row0 + (j - copy.cached);
-        const int64_t off = B::block_of(c) + B::piece_of(lane_l, c);
-        valid |= ok || j < copy.cached ? (1u << c) : 0u;
-        if (!HALF || !v)
-          copy_to_lds_16B((ok ? a.k_new + cr * a.k_st + copy.h * a.k_sh : a.k_cache) + off,
-                          __builtin_amdgcn_readfirstlane(dst + c * 1024));
-        if (!HALF || v)
-          copy_to_lds_16B((ok ? a.v_new + cr * a.v_st + copy.h * a.v_sh : a.v_cache) + off,
-                          __builtin_amdgcn_readfirstlane(dst + B::G::kTileBytes + c * 1024));
-      }
-      if (HALF && !v) valid = B::kAllValid;
+    for (int c = 0; c < B::L; ++c) {
+      const int j = kb + B::row_of(lane_l, c);
+      const bool ok = j >= copy.cached && j < copy.key_end;
+      const int64_t cr = copy.chunk_row0 + (j - copy.cached);
+      const int64_t off = B::block_of(c) + B::piece_of(lane_l, c);
+      valid |= ok || j < copy.cached ? (1u << c) : 0u;
+      if (!HALF || !v)
+        copy_to_lds_16B((ok ? a.k_new + cr * a.k_st + copy.h * a.k_sh : a.k_cache) + off,
+                        __builtin_amdgcn_readfirstlane(dst + c * 1024));
+      if (!HALF || v)
+        copy_to_lds_16B((ok ? a.v_new + cr * a.v_st + copy.h * a.v_sh : a.v_cache) + off,
+                        __builtin_amdgcn_readfirstlane(dst + B::G::kTileBytes + c * 1024));
     }
-    const int id = __builtin_amdgcn_readfirstlane(block_id);
-    const bool ok = static_cast<uint32_t>(id) < a.num_blocks_u32;
-    const int64_t bh = (ok ? static_cast<int64_t>(id) : 0) * a.num_kv_heads + copy.h;
-    const int64_t at = ((bh << a.bs_log2) + (kb & ((1 << a.bs_log2) - 1))) * D;
-    // (a scalar load: a vector load's wait would be one for the copies too)
-    const auto* scales = reinterpret_cast<const __attribute__((address_space(4))) float*>(
-        reinterpret_cast<uintptr_t>(a.kv_scales + 2 * bh));
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool is_v = HALF ? v : n == 1;
-      scale[n] = ok ? scales[is_v ? 1 : 0] : 0.f;
-#pragma unroll
-      for (int c = 0; c < CL; ++c)
-        copy_to_lds_16B_sv((is_v ? a.v_cache : a.k_cache) + at + c * 1024, copy.lane * 16,
-                           __builtin_amdgcn_readfirstlane(code_dst + (is_v ? code_step : 0) + c * 1024));
-    }
-    return valid;
+    return HALF && !v ? B::kAllValid : valid;
   }
 
-  // Turns the landed codes into their rows of the sub-tile at s_sub (an id
-  // outside the pool: zeros).
+  // Turns the landed codes into their rows of the sub-tile at s_sub.
   __device__ __forceinline__ void settle(char* s_sub, const char* s_mix, int lane, bool v) const {
     if (rows == 0) return;
     asm volatile("" : "+v"(lane));  // (these addresses are not kept through the key loop)
+    const int row = lane >> 2, piece = (lane & 3) * 2, sw = piece_swizzle<8>(row);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bool is_v = HALF ? v : n == 1;
       char* tile = s_sub + (is_v ? B::G::kTileBytes : 0);
-      const char* from = rows < kTile ? s_mix + (is_v ? kCodeBytes : 0) : tile;
-      u32x4 codes[CL];  // (all read before a row is written over them)
-#pragma unroll
-      for (int c = 0; c < CL; ++c) codes[c] = *reinterpret_cast<const u32x4*>(from + c * 1024 + lane * 16);
+      u32x4 x[CL];  // (in place: all read before a row is written over them)
 #pragma unroll
       for (int c = 0; c < CL; ++c) {
-        const int row = (c * 64 + lane) / (D / 16), dim = lane % (D / 16) * 16;
+        if constexpr (kRegs) x[c] = codes[n][c];
+        else x[c] = *reinterpret_cast<const u32x4*>((rows < kTile ? s_mix + (is_v ? kCodeBytes : 0) : tile) + c * 1024 + lane * 16);
+      }
+#pragma unroll
+      for (int c = 0; c < CL; ++c) {
         u32x2 w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = scale[n] > 0.f ? fp8_unpack4<DTYPE>(codes[c][i], scale[n]) : u32x2{0, 0};
+        for (int i = 0; i < 4; ++i) w[i] = fp8_unpack4<DTYPE>(x[c][i], scale[n]);
         if (row < rows) {
-          char* at = tile + dim / 64 * 2048 + row * 128;
-          const int piece = dim % 64 / 8, sw = piece_swizzle<8>(row);
+          char* at = tile + c * 2048 + row * 128;
           *reinterpret_cast<u32x4*>(at + ((piece ^ sw) << 4)) = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
           *reinterpret_cast<u32x4*>(at + (((piece + 1) ^ sw) << 4)) = u32x4{w[2][0], w[2][1], w[3][0], w[3][1]};
         }
@@ -338,7 +361,9 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
   // ---- the key stream: this wave's share of stage k's copies into buffer st
   SubTileCopy<DTYPE, D> copy{a, s_ids, h, cached, key_end, chunk_row0, lane, {}, {}, {}};
   copy.init();
-  [[maybe_unused]] Fp8SubTile<DTYPE, D, Tr::kHalfSubs> fp8;
+  using Fp8 = Fp8SubTile<DTYPE, D, Tr::kHalfSubs>;
+  constexpr bool kCodeRegs = Tr::kFp8 && Fp8::kRegs;
+  [[maybe_unused]] Fp8 fp8;
   int win_blk0 = 0;
   const int su = Tr::kHalfSubs ? wave >> 1 : wave;  // the wave's sub-tile
   auto stage_id = [&](int k) __attribute__((always_inline)) {
@@ -348,7 +373,9 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
     const int kb = k * Tr::kStageTokens + su * kTile;
     const uint32_t dst = lds0 + st * Tr::kStageBytes + su * Tr::kSubBytes;
     if constexpr (Tr::kFp8) {
-      return fp8.fetch(copy, kb, win_blk0, dst, lds0 + Tr::kMixOffset, id, Tr::kHalfSubs && (wave & 1));
+      const bool v = Tr::kHalfSubs && (wave & 1);
+      if constexpr (!kCodeRegs) fp8.fetch(copy, kb, dst, lds0 + Tr::kMixOffset, id, v);
+      return fp8.copy_rows(copy, kb, win_blk0, dst, id, v);
     } else if constexpr (Tr::kHalfSubs) {
       if (wave & 1) return copy.template copy<false, true>(kb, win_blk0, dst, id);
       copy.template copy<true, false>(kb, win_blk0, dst, id);
@@ -357,18 +384,23 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
       return copy.copy(kb, win_blk0, dst, id);
     }
   };
+  // The codes of stage k into registers (kCodeRegs): free once a stage landed.
+  auto fetch_codes = [&](int k, int id) __attribute__((always_inline)) {
+    if constexpr (kCodeRegs) fp8.fetch(copy, k * Tr::kStageTokens + su * kTile, 0, 0, id, Tr::kHalfSubs && (wave & 1));
+  };
   // Waits for this wave's copies of a stage (the next stage's may stay in
   // flight) and meets the other waves: the stage is whole, and every wave has
   // read what it needs of the one before. V slots of keys that were not
   // loaded read pool row 0 instead: they are cleared first (P is 0 there, but
-  // 0 * NaN would not be).
-  auto land = [&](int st, unsigned ok, bool more) __attribute__((always_inline)) {
+  // 0 * NaN would not be). next_codes: 8-bit codes, loads those of the stage after.
+  auto land = [&](int st, unsigned ok, bool more, auto next_codes) __attribute__((always_inline)) {
     if constexpr (Tr::kFp8) wait_vmcnt<0>();  // (one stage in flight)
     else wait_vmcnt_groups<Tr::kWaveLoads, 1>(more);
     asm volatile("" ::: "memory");
     if constexpr (Tr::kFp8)
       fp8.settle(s_lds + st * Tr::kStageBytes + su * Tr::kSubBytes, s_lds + Tr::kMixOffset, lane,
                  Tr::kHalfSubs && (wave & 1));
+    next_codes();
     if (__builtin_amdgcn_ballot_w64(ok != copy.kAllValid) != 0) {
       char* vdst = s_lds + st * Tr::kStageBytes + su * Tr::kSubBytes + Tr::kTileBytes;
 #pragma unroll
@@ -445,10 +477,11 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
     __syncthreads();  // block ids of the window visible; previous window's stages released
     const int k0 = first / Tr::kStageTokens;
     const int ns = (min(key_end, win0 + win_tokens) - first + Tr::kStageTokens - 1) / Tr::kStageTokens;
+    fetch_codes(k0, stage_id(k0));
     const unsigned ok = issue(k0, 0, stage_id(k0));
     unsigned ok_next = 0;
     if (!Tr::kFp8 && ns > 1) ok_next = issue(k0 + 1, 1, stage_id(k0 + 1));
-    land(0, ok, ns > 1);
+    land(0, ok, ns > 1, [&] { if (ns > 1) fetch_codes(k0 + 1, stage_id(k0 + 1)); });
     if (Tr::kFp8 && ns > 1) ok_next = issue(k0 + 1, 1, stage_id(k0 + 1));
 
     // this wave's tiles that some row of it sees, and the stages full of them
@@ -467,9 +500,11 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
       qk(0, KB, s[0]);
       auto step = [&](auto st_c) __attribute__((always_inline)) {
         constexpr int ST = decltype(st_c)::value;
+        [[maybe_unused]] int code_id = 0;
+        if constexpr (kCodeRegs) code_id = stage_id(k0 + i + 2);
         do_tile(set_key + i * T * SETS * 32, s[0], IntC<1>{}, s[1], [&] { read_k(ST, kTileStep); });
         read_v(ST, kTileStep);
-        if (i + 1 < ns) land(ST ^ 1, ok_next, false);
+        if (i + 1 < ns) land(ST ^ 1, ok_next, false, [&] { if (i + 2 < ns) fetch_codes(k0 + i + 2, code_id); });
         const int id = stage_id(k0 + i + 2);
         do_tile(set_key + (i * T + 1) * SETS * 32, s[1], IntC<1>{}, s[0], [&] { read_k(ST ^ 1, 0); });
         read_v(ST ^ 1, 0);
@@ -494,7 +529,8 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
         qk(0, KB, s);
         do_tile(set_key + (i * T + t) * SETS * 32, s, IntC<0>{}, s, [] {});
       }
-      if (i + 1 < ns) land(st ^ 1, ok_next, false);
+      if (i + 1 < ns)
+        land(st ^ 1, ok_next, false, [&] { if (i + 2 < ns) fetch_codes(k0 + i + 2, stage_id(k0 + i + 2)); });
       if (i + 2 < ns) ok_next = issue(k0 + i + 2, st, stage_id(k0 + i + 2));
       asm volatile("" ::: "memory");
     }
