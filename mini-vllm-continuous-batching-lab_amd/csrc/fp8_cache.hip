@@ -30,7 +30,8 @@ namespace {
 // is place o of it, or -1. Built by inserting every token's block into a hash
 // table (open addressing, at least twice as many entries as tokens) whose
 // first inserter takes the next item. The order of the items depends on the
-// atomics; nothing that is computed from them does.
+// atomics; nothing that is computed from them does. Up to 2048 tokens one work
+// group does it in LDS in one launch; beyond, four launches over the tokens.
 constexpr int kFp8PlanThreads = 1024;
 constexpr int kFp8PlanSmall = 2048;  // tokens one work group plans in LDS
 
@@ -158,7 +159,9 @@ __global__ __launch_bounds__(256) void fp8_plan_place_kernel(Fp8PlanArgs a) {
     if (slot < 0 || slot >= a.total_slots) continue;
     const int32_t block = static_cast<int32_t>(slot >> a.bs_log2);
     uint32_t h = hash_block(static_cast<uint32_t>(block)) & a.mask;
-    while (a.keys[h] != block) h = (h + 1) & a.mask;  // (ends: the block was inserted)
+    int32_t seen;  // (ends: the table has empty entries; the block was inserted)
+    while ((seen = a.keys[h]) != block && seen != -1) h = (h + 1) & a.mask;
+    if (seen == -1) continue;
     const int64_t cell = (static_cast<int64_t>(a.keys[static_cast<int64_t>(a.mask) + 1 + h]) << a.bs_log2) +
                          (slot & ((1 << a.bs_log2) - 1));
     if (atomicMax(&a.table[cell], static_cast<int32_t>(t)) >= 0) atomicAdd(&a.status[1], 1);
@@ -252,19 +255,33 @@ __device__ __forceinline__ float elem16(const Row16& r, int i) {
 __device__ __forceinline__ bool finite_bits(uint32_t abs_bits) { return abs_bits < 0x7f800000u; }
 
 // max over the wave (all lanes get it)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t x) {
+  const uint32_t y = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), CTRL, 0xf, 0xf, true));
+  return x > y ? x : y;
+}
 __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) {
-    const uint32_t y = static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), s));
-    x = x > y ? x : y;
-  }
-  return x;
+  x = dpp_umax<0xb1>(x);   // lane ^ 1
+  x = dpp_umax<0x4e>(x);   // lane ^ 2
+  x = dpp_umax<0x141>(x);  // 7 - lane of 8
+  x = dpp_umax<0x140>(x);  // 15 - lane of 16
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = r[0] > r[1] ? r[0] : r[1];
+  const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return s[0] > s[1] ? s[0] : s[1];
 }
 
 // A unit is one (touched block, kv head, K or V): block_size x D values, a
 // thread holds 16 of one row. Units of up to 256 threads share a work group
-// of 256 (FIT); larger ones go over the rows twice, the second time from the
-// caches.
+// of 256 (FIT): one pass, the rows kept in registers between the maximum and
+// the codes; larger ones go over the rows twice, the second time from the
+// caches. A decode step's append is bound by the launch and four rounds of
+// dependent loads (plan words; row, position and scale; cos and sin; codes
+// that shrink): 3.0 us for one row at 14 / 2 x 64 with the query's rotation,
+// 4.2 for 64 (3.25 and 4.45 with the plan's words in two rounds and the wave's
+// maximum through LDS). A prompt's is bound by its bytes: 31.2 us for 166 MB
+// (9 k tokens at 28 / 4 x 128, rotation and returned key), 5.3 TB/s, a large
+// copy's rate.
 template <int DTYPE, int D, bool FIT>
 __device__ __forceinline__ void write_units(const Fp8WriteArgs& a) {
   constexpr int kPer = D / 16;  // threads per row
@@ -275,26 +292,32 @@ __device__ __forceinline__ void write_units(const Fp8WriteArgs& a) {
   const int lt = threadIdx.x & (width - 1);
   const int sub = threadIdx.x / width;
   const int wave = threadIdx.x >> 6;
-  const int items = min(a.status[3], a.max_items);
-  const int64_t units = static_cast<int64_t>(items) * a.num_kv_heads * 2;
+  const int64_t bound = static_cast<int64_t>(a.max_items) * a.num_kv_heads * 2;
   const float limit = fp8_limit<DTYPE>();
   // (every thread of the work group goes through the same number of rounds:
   // the barriers below)
-  for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * per_group; u0 < units;
+  for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * per_group; u0 < bound;
        u0 += static_cast<int64_t>(a.write_groups) * per_group) {
     const int64_t u = u0 + sub;
-    const bool live = u < units;
+    const bool live = u < bound;
     const int j = static_cast<int>(u & 1);  // 0: K, 1: V
     const int64_t ih = live ? u >> 1 : 0;
     const int h = static_cast<int>(ih % a.num_kv_heads);
     const int64_t item = ih / a.num_kv_heads;
-    const int64_t block = a.items[item];
-    const bool ok = live && block >= 0 && block < a.num_blocks;
+    // the plan's words in one round of loads, the number of items among them:
+    // what lies behind the last item is read and not used
     const int32_t* tab = a.table + (item << a.bs_log2);
+    const int64_t block = a.items[item];
+    const int first = tab[0];
+    int tok = FIT ? tab[lt / kPer] : 0;
+    const int items = a.status[3];
+    asm volatile("" : "+v"(tok) : "v"(first), "v"(static_cast<int>(block)), "s"(items));
+    if (u0 >= static_cast<int64_t>(items) * a.num_kv_heads * 2) break;
+    const bool ok = live && item < items && block >= 0 && block < a.num_blocks;
     const int64_t tile = (block * a.num_kv_heads + h) << a.bs_log2;
     float* const scale_at = a.scales + (block * a.num_kv_heads + h) * 2 + j;
     uint8_t* const cache = j ? a.v_cache : a.k_cache;
-    const bool anew = tab[0] >= 0;
+    const bool anew = first >= 0;
     const float old = ok && !anew ? *scale_at : 0.f;
 
     // the rows of this thread: row (it * width + lt) / kPer, piece lt % kPer
@@ -332,11 +355,9 @@ __device__ __forceinline__ void write_units(const Fp8WriteArgs& a) {
     };
 
     Row16 x;
-    int tok = -1;
     uint32_t amax = 0;
     if constexpr (FIT) {
-      tok = ok ? token_of(lt) : -1;
-      if (tok >= a.num_tokens) tok = -1;
+      if (!ok || tok >= a.num_tokens) tok = -1;
       if (tok >= 0) {
         x = load_row(tok, lt);
         amax = row_max(x);
