@@ -30,9 +30,10 @@ same metadata; without one they make it, and find it again for the step's other
 layers by their unmodified metadata tensors, as ``paged_attention_gpu`` does. A
 plan may be used on any stream; a decode or prefill plan holds the workspace of
 its merge, so calls with the same one have to be ordered among themselves (calls
-with plans of their own need not be). While a stream is being captured into a
-graph, a call without a plan records the planning too, and its checks raise from
-``check_deferred()``; a plan made outside the graph has to outlive it.
+with plans of their own, or without ``plan`` on different streams, need not be).
+While a stream is being captured into a graph, a call without a plan records the
+planning too, and its checks raise from ``check_deferred()``; a plan made outside
+the graph has to outlive it, and one made inside serves that capture only.
 """
 
 from __future__ import annotations
@@ -100,6 +101,11 @@ class _Plan:
             current = torch.cuda.current_stream(self.device)
             for t in self.buffers:
                 t.record_stream(current)
+
+    def _check_capture(self) -> None:
+        """A plan recorded into a graph holds nothing until that graph is replayed."""
+        if self.capture and self.capture != _gpu._capture_id(self.device):
+            raise RuntimeError("the plan was made inside a graph's capture: it serves that capture only")
 
 
 def _seen_plan(name: str, *tensors):
@@ -261,7 +267,8 @@ def _append(who, query, key, value, positions, cos, sin, key_cache, value_cache,
     known = plan
     if known is None:
         known = _seen_plan("fp8_write", *((slot_mapping,) if cos is None else (slot_mapping, positions)))
-    if known is not None and native is not None and slot_mapping.shape == (known.num_tokens,):
+    if (known is not None and native is not None and not known.capture
+            and slot_mapping.shape == (known.num_tokens,)):
         stream = _gpu._stream(known.device)
         if stream == known.stream and (cos is None or known.max_positions):
             done = native.write(known.words, query, key, value, cos, sin, key_cache, value_cache,
@@ -303,6 +310,7 @@ def _append(who, query, key, value, positions, cos, sin, key_cache, value_cache,
                                positions if rope else None, max_pos)
         assert (plan.num_tokens, plan.block_size, plan.num_blocks, plan.device) == (
             num_tokens, block_size, num_blocks, device), "the plan is of another step or pool"
+        plan._check_capture()
         assert not rope or plan.max_positions == max_pos, (
             f"the plan's positions were checked against {plan.max_positions} rows, not {max_pos}"
         )
@@ -420,6 +428,7 @@ class Fp8DecodePlan(_Plan):
 
     plan: _gpu.DecodePlan = None
     key: tuple = ()  # (num_seqs, block_size, num_blocks, head_dim, num_kv_heads)
+    owner: Optional[torch.cuda.Stream] = None  # `stream`
     workspaces: dict = field(default_factory=dict)
 
     def workspace(self, num_q_heads: int, head_dim: int) -> Optional[torch.Tensor]:
@@ -429,6 +438,8 @@ class Fp8DecodePlan(_Plan):
             ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
             self.workspaces[num_q_heads] = ws
             if ws is not None:
+                if _gpu._stream(self.device) != self.stream and not _gpu._capturing():
+                    ws.record_stream(self.owner)  # (calls on the plan's stream do not)
                 self.buffers += (ws,)
         return self.workspaces[num_q_heads]
 
@@ -510,7 +521,8 @@ def plan_fp8_decode(
         made = _gpu.DecodePlan(buf[:n_work], buf[n_work:n_work + n_ids],
                                buf[n_work + n_ids:n_work + n_ids + n_units], groups, parts, tokens)
         return Fp8DecodePlan(device, (buf,), _gpu._stream(device), capture, plan=made,
-                             key=(num_seqs, block_size, num_blocks, head_dim, num_kv_heads))
+                             key=(num_seqs, block_size, num_blocks, head_dim, num_kv_heads),
+                             owner=torch.cuda.current_stream(device))
 
 
 def hip_fp8_decode_attention(
@@ -535,7 +547,7 @@ def hip_fp8_decode_attention(
     """
     native = _hip.native_fp8
     known = plan if plan is not None else _seen_plan("fp8_decode", block_table, kv_len_after)
-    if known is not None and native is not None and known.words is not None:
+    if known is not None and native is not None and known.words is not None and not known.capture:
         stream = _gpu._stream(known.device)
         if stream == known.stream:
             output = native.decode(known.words, query, key_cache, value_cache, kv_scales, block_table,
@@ -564,10 +576,11 @@ def hip_fp8_decode_attention(
         output = torch.empty_like(query, memory_format=torch.contiguous_format)
         if num_seqs == 0:
             return output
+        stream = _gpu._stream(device)
         if plan is None:
             capture = _gpu._capture_id(device)
             name = "fp8_decode_graph" if capture else "fp8_decode"
-            extra = (block_size, num_blocks, device, head_dim, num_kv_heads, capture)
+            extra = (block_size, num_blocks, device, head_dim, num_kv_heads, capture, stream)
             plan = _gpu._cache_get(name, (block_table, kv_len_after), extra)
             if plan is None:
                 plan = plan_fp8_decode(block_table, kv_len_after, block_size, num_blocks, device,
@@ -575,10 +588,10 @@ def hip_fp8_decode_attention(
                 _gpu._cache_put(name, (block_table, kv_len_after), extra, plan)
         assert plan.key == (num_seqs, block_size, num_blocks, head_dim, num_kv_heads) and (
             plan.device == device), "the plan is of another step or pool"
+        plan._check_capture()
         p = plan.plan
         if p.num_groups == 0:
             return output
-        stream = _gpu._stream(device)
         plan._used(stream)
         ws = plan.workspace(num_q_heads, head_dim)
         query, qp, q_st, q_sh = _gpu._row_args(query)
@@ -716,7 +729,7 @@ def hip_fp8_prefill_attention(
             if plan is None:
                 cached, qlens = _gpu._host_lengths(cached_len_before, query_len)
                 extra = (tuple(rows), tuple(cached), tuple(qlens), block_size, num_blocks,
-                         num_q_heads, num_kv_heads, head_dim, dtype, device)
+                         num_q_heads, num_kv_heads, head_dim, dtype, device, stream)
                 plan = _gpu._cache_get("fp8_prefill", (block_table,), extra)
                 if plan is None:
                     plan = plan_fp8_prefill(block_table, rows, cached, qlens, block_size, num_blocks,

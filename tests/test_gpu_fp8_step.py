@@ -351,3 +351,108 @@ def test_native_calls_equal_the_wrappers(form, monkeypatch):
         gpu.invalidate_cached_metadata()
     assert len(results[0]) == len(results[1]) == 24
     assert all(torch.equal(bits(a), bits(b)) for a, b in zip(*results))
+
+
+def _decode_set(n, seed, hq=14, hkv=2, d=64, bs=16, dtype=torch.bfloat16):
+    num_blocks = -(-n // bs)
+    kc, vc, sc = fp8_util.random_pool(num_blocks, hkv, bs, d, seed, DEV)
+    q = torch.randn(1, hq, d, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+    return q, kc, vc, sc, torch.arange(num_blocks, device=DEV)[None], torch.tensor([n], device=DEV), bs
+
+
+def test_one_steps_calls_on_two_streams():
+    """Two layers of a step on a stream each, at once, without a plan given: neither
+    merges in the other's workspace."""
+    layers = [list(_decode_set(6000, i)) for i in range(2)]
+    layers[1][4:6] = layers[0][4:6]  # the step's table and lengths
+    want = []
+    for layer in layers:
+        gpu.invalidate_cached_metadata()
+        want.append(fp8.hip_fp8_decode_attention(*layer))
+    streams = [torch.cuda.Stream() for _ in layers]
+    torch.cuda.synchronize()
+    gpu.invalidate_cached_metadata()
+    outs = [[], []]
+    for i, stream in enumerate(streams):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                outs[i].append(fp8.hip_fp8_decode_attention(*layers[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(bits(o), bits(want[i])) for o in outs[i])
+
+
+def test_plan_first_used_on_another_stream():
+    layer = _decode_set(6000, 3)
+    want = fp8.hip_fp8_decode_attention(*layer)
+    kc, bt, kv, bs = layer[1], *layer[4:]
+    plan = fp8.plan_fp8_decode(bt, kv, bs, kc.shape[0], DEV, kc.shape[3], kc.shape[1])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        first = fp8.hip_fp8_decode_attention(*layer, plan=plan)
+    torch.cuda.current_stream().wait_stream(side)
+    second = fp8.hip_fp8_decode_attention(*layer, plan=plan)
+    del plan  # (its memory waits for the calls)
+    with torch.cuda.stream(side):
+        junk = [torch.full((1 << 20,), 7, dtype=torch.uint8, device=DEV) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(bits(first), bits(want)) and torch.equal(bits(second), bits(want)), len(junk)
+
+
+def test_plan_of_a_capture_serves_it_only():
+    layer = _decode_set(300, 5)
+    kc, vc, sc, bt, kv, bs = layer[1:]
+    nb, hkv, _, d = kc.shape
+    slots = torch.tensor([16, 17], device=DEV)
+    k, v = (torch.randn(2, hkv, d, device=DEV).to(torch.bfloat16) for _ in range(2))
+    pool = [x.clone() for x in (kc, vc, sc)]
+    fp8.hip_fp8_cache_write(k, v, *pool, slots, bs)
+    want = fp8.hip_fp8_decode_attention(layer[0], *pool, bt, kv, bs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        write = fp8.plan_fp8_write(slots, bs, nb, DEV)
+        decode = fp8.plan_fp8_decode(bt, kv, bs, nb, DEV, d, hkv)
+        fp8.hip_fp8_cache_write(k, v, kc, vc, sc, slots, bs, plan=write)
+        out = fp8.hip_fp8_decode_attention(*layer, plan=decode)
+    gid = gpu.last_capture_id()
+    with pytest.raises(RuntimeError, match="that capture only"):
+        fp8.hip_fp8_cache_write(k, v, kc, vc, sc, slots, bs, plan=write)
+    with pytest.raises(RuntimeError, match="that capture only"):
+        fp8.hip_fp8_decode_attention(*layer, plan=decode)
+    for _ in range(3):
+        graph.replay()
+        gpu.check_deferred(gid)
+        assert torch.equal(bits(out), bits(want))
+    gpu.clear_deferred(gid)
+
+
+def test_pools_past_4_gib():
+    """Blocks whose offsets pass 32 bits: every call equals the same one on a small pool."""
+    hq, hkv, d, bs, dtype = 4, 2, 128, 16, torch.bfloat16
+    num_blocks = (5 << 30) // (hkv * bs * d)
+    far = [num_blocks - 1, 3, (4 << 30) // (hkv * bs * d), num_blocks - 2, (2 << 30) // (hkv * bs * d) + 1]
+    g = torch.Generator().manual_seed(1)
+    n, new = 70, 9
+    k, v = (torch.randn(n, hkv, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    q = torch.randn(new, hq, d, generator=g).to(dtype).to(DEV)
+    got = []
+    for blocks, count in ((list(range(5)), 5), (far, num_blocks)):
+        kc, vc = (torch.zeros(count, hkv, bs, d, dtype=torch.uint8, device=DEV).view(fp8.FP8_DTYPE) for _ in range(2))
+        sc = torch.zeros(count, hkv, 2, device=DEV)
+        table = torch.tensor([blocks], device=DEV)
+        slots = torch.tensor([blocks[p // bs] * bs + p % bs for p in range(n)], device=DEV)
+        fp8.hip_fp8_cache_write(k, v, kc, vc, sc, slots, bs)
+        fp8.hip_fp8_cache_write(3 * k[-2:], v[-2:], kc, vc, sc, slots[-2:], bs)
+        res = [fp8.hip_fp8_decode_attention(q[:1], kc, vc, sc, table, torch.tensor([n], device=DEV), bs),
+               fp8.hip_fp8_prefill_attention(q, k[:new], v[:new], kc, vc, sc, table, [0], [n], [new], bs),
+               *fp8.gather_fp8_prefix_kv(kc, vc, sc, table, [n], [0], bs, dtype)]
+        at = torch.tensor(blocks, device=DEV)
+        res += [kc.view(torch.uint8)[at], vc.view(torch.uint8)[at], sc[at]]
+        assert (sc[at] > 0).all()
+        torch.cuda.synchronize()
+        got.append([r.cpu() for r in res])
+        del kc, vc, sc
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
