@@ -407,9 +407,16 @@ __global__ __launch_bounds__(kDwWaves * 64) __attribute__((amdgpu_waves_per_eu(2
 // 8.5, in 4 9.2; 16 x 8k-32k one group per CU 19.8, two 21.6; 128 x 512-4096 at
 // 28 / 4 x 128 uncut, two groups per CU 52, cut for three 63.5; 256 x
 // lognormal(300) 11.3 cut for three, 25.8 uncut.
+//
+// One work group makes the plan. It is bound by its chain of barriers and
+// reductions, so totals are taken in registers (lane permutes), a group finds its
+// piece by bisection and its rank by counting sizes: 10-12 us for up to 128
+// sequences and 512 groups, 20 for 1000 sequences (23-48 with atomics for the
+// totals and every pair of groups compared), plus 4 for the id lists.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kPlanDealt = 1024;    // groups of a launch that is dealt, at most
+constexpr int kPlanSeqs = 4096;     // sequences whose tiles are kept in LDS
 constexpr int kPlanMaxParts = 128;  // pieces of a sequence
 constexpr int kPlanMinTiles = 4;    // tiles of a piece: one for each wave
 constexpr float kHbmBytesPerUs = 6.3e6f;
@@ -439,14 +446,39 @@ __device__ __forceinline__ int64_t int_at(const void* p, int i64, int64_t i) {
   return i64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) x += __shfl_xor(x, s);
-  return x;
+// A reduction over the wave's lanes (all get it), and over groups of 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ int dpp_lane(int x) {
+  return __builtin_amdgcn_mov_dpp(x, CTRL, 0xf, 0xf, true);
 }
-__device__ __forceinline__ int wave_max(int x) {
+template <class Op>
+__device__ __forceinline__ int row_reduce(int x, Op op) {
+  x = op(x, dpp_lane<0xb1>(x));     // lane ^ 1
+  x = op(x, dpp_lane<0x4e>(x));     // lane ^ 2
+  x = op(x, dpp_lane<0x141>(x));    // 7 - lane of 8
+  return op(x, dpp_lane<0x140>(x)); // 15 - lane of 16
+}
+template <class Op>
+__device__ __forceinline__ int wave_reduce(int x, Op op) {
+  x = row_reduce(x, op);
+  const auto r = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(x), static_cast<uint32_t>(x), false, false);
+  x = op(static_cast<int>(r[0]), static_cast<int>(r[1]));
+  const auto s = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(x), static_cast<uint32_t>(x), false, false);
+  return op(static_cast<int>(s[0]), static_cast<int>(s[1]));
+}
+struct Sum {
+  __device__ int operator()(int a, int b) const { return a + b; }
+};
+struct Max {
+  __device__ int operator()(int a, int b) const { return max(a, b); }
+};
+// The sum of the lanes up to and with this one.
+__device__ __forceinline__ int wave_scan(int x, int lane) {
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) x = max(x, __shfl_xor(x, s));
+  for (int s = 1; s < 64; s <<= 1) {
+    const int y = __shfl_up(x, s);
+    if (lane >= s) x += y;
+  }
   return x;
 }
 
@@ -458,163 +490,186 @@ __device__ __forceinline__ int planned_tiles(const Fp8DecodePlanArgs& a, int64_t
 }
 
 __global__ __launch_bounds__(kPlanThreads) void fp8_decode_plan_kernel(Fp8DecodePlanArgs a) {
-  __shared__ int s_a[kPlanWaves];
+  __shared__ int s_tiles[kPlanSeqs];        // tiles of the first sequences
+  __shared__ int s_red[6][kPlanWaves];      // totals of the waves
+  __shared__ int4 s_try[kPlanWaves];        // a tried L, its groups / H, pieces, longest piece
   __shared__ float s_cost[kPlanWaves];
-  __shared__ int s_l[kPlanWaves];
-  __shared__ int s_bad, s_short, s_min, s_total, s_most, s_live, s_base;
-  __shared__ int s_size[kPlanDealt];
-  __shared__ int4 s_item[kPlanDealt];  // sequence, piece, pieces, kv head
+  __shared__ int s_first[kPlanThreads];     // a sequence's first piece; places by size
+  __shared__ int4 s_item[2 * kPlanDealt];   // the groups to deal, as in the work list
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int H = a.num_kv_heads, C = a.cu_count;
-  if (tid == 0) {
-    s_bad = s_short = 0;
-    s_min = INT_MAX;
-    s_total = s_most = s_live = 0;
-    s_base = 0;
-  }
-  __syncthreads();
+  auto tiles = [&](int b) {
+    return b < kPlanSeqs ? s_tiles[b] : planned_tiles(a, int_at(a.kv_len, a.kv_i64, b));
+  };
   // ---- lengths: checks, all tiles, the most tiles of a sequence
-  {
-    int total = 0, most = 0, live = 0, bad = 0, over = 0, low = INT_MAX;
-    for (int b = tid; b < a.num_seqs; b += kPlanThreads) {
-      const int64_t kv = int_at(a.kv_len, a.kv_i64, b);
-      low = min(low, static_cast<int>(kv < INT_MIN ? INT_MIN : kv > INT_MAX ? INT_MAX : kv));
-      bad += kv < 1;
-      over += kv > (static_cast<int64_t>(a.max_blocks) << a.bs_log2);
-      const int t = planned_tiles(a, kv);
-      total += t;
-      live += t > 0;
-      most = max(most, t);
-    }
-    if (bad) atomicAdd(&s_bad, bad);
-    if (over) atomicAdd(&s_short, over);
-    atomicMin(&s_min, low);
-    atomicAdd(&s_total, total);
-    atomicAdd(&s_live, live);
-    atomicMax(&s_most, most);
+  int red[6] = {0, 0, 0, 0, 0, -INT_MAX};  // tiles, most, sequences, too short, too long, -shortest
+  for (int b = tid; b < a.num_seqs; b += kPlanThreads) {
+    const int64_t kv = int_at(a.kv_len, a.kv_i64, b);
+    const int t = planned_tiles(a, kv);
+    if (b < kPlanSeqs) s_tiles[b] = t;
+    red[0] += t;
+    red[1] = max(red[1], t);
+    red[2] += t > 0;
+    red[3] += kv < 1;
+    red[4] += kv > (static_cast<int64_t>(a.max_blocks) << a.bs_log2);
+    red[5] = max(red[5], -static_cast<int>(kv < -INT_MAX ? -INT_MAX : kv > INT_MAX ? INT_MAX : kv));
   }
   for (int i = tid; i < a.num_seqs * H; i += kPlanThreads) a.counters[i] = 0;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    const int v = k == 1 || k == 5 ? wave_reduce(red[k], Max()) : wave_reduce(red[k], Sum());
+    if (lane == 0) s_red[k][wave] = v;
+  }
   __syncthreads();
-  const int total = s_total, most = s_most;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    const int v = s_red[k][lane & (kPlanWaves - 1)];
+    red[k] = k == 1 || k == 5 ? row_reduce(v, Max()) : row_reduce(v, Sum());
+  }
+  __syncthreads();
+  const int total = red[0], most = red[1];
   // ---- the piece bound L: every wave tries one, 16 over the whole range, then
   // 16 around the best
-  int best = max(most, 1);
-  int groups = 0, parts = 1, longest = 1;
+  int best = 1, groups = 0, parts = 1, longest = 1;
   if (most > 0) {
     const int least = min(most, max(kPlanMinTiles, (most + kPlanMaxParts - 1) / kPlanMaxParts));
     int hi = most, lo = least;
-    for (int round = 0; round < 3; ++round) {
-      // round 2: the chosen L once more, for its groups, pieces and size
+    for (int round = 0; round < 2; ++round) {
       int L;
-      if (round == 0) L = static_cast<int>(most * exp2f(log2f(static_cast<float>(least) / most) * wave / (kPlanWaves - 1)) + 0.5f);
-      else if (round == 1) L = hi - static_cast<int>(static_cast<int64_t>(hi - lo) * wave / (kPlanWaves - 1));
-      else L = best;
+      if (round == 0)
+        L = static_cast<int>(most * __builtin_amdgcn_exp2f(__builtin_amdgcn_logf(static_cast<float>(least) / most) *
+                                                            wave / (kPlanWaves - 1)) + 0.5f);
+      else
+        L = hi - static_cast<int>(static_cast<uint32_t>(hi - lo) * wave / (kPlanWaves - 1));
       L = min(max(L, least), most);
       int n = 0, np_most = 1, piece = 1;
       for (int b = lane; b < a.num_seqs; b += 64) {
-        const int t = planned_tiles(a, int_at(a.kv_len, a.kv_i64, b));
-        const int np = (t + L - 1) / L;
+        const uint32_t t = tiles(b);
+        const uint32_t np = (t + L - 1) / static_cast<uint32_t>(L);
         n += np;
-        np_most = max(np_most, np);
-        if (np > 0) piece = max(piece, (t + np - 1) / np);
+        np_most = max(np_most, static_cast<int>(np));
+        if (np > 0) piece = max(piece, static_cast<int>((t + np - 1) / np));
       }
-      n = wave_sum(n);
-      np_most = wave_max(np_most);
-      piece = wave_max(piece);
-      if (round == 2) {
-        groups = n * H;
-        parts = np_most;
-        longest = piece;
-        break;
-      }
+      n = wave_reduce(n, Sum());
+      np_most = wave_reduce(np_most, Max());
+      piece = wave_reduce(piece, Max());
       const float G = static_cast<float>(n) * H, mean = static_cast<float>(total) * H / C;
       float busiest = piece;
       if (G > 3.f * C) busiest = mean * 1.1f + piece;
       else if (G > C) busiest = fmaxf(busiest, mean * 1.05f);
       const float all = static_cast<float>(total) * H * a.tile_bytes / kHbmBytesPerUs;
       const float cu = busiest * a.tile_bytes / a.cu_bytes_per_us;
-      float cost = sqrtf(sqrtf(all * all * all * all + cu * cu * cu * cu)) +
-                   (np_most > 1 ? kMergeUs + kMergePartUs * (static_cast<float>(n) / s_live - 1.f) * G / C : 0.f) +
+      float cost = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(all * all * all * all + cu * cu * cu * cu)) +
+                   (np_most > 1 ? kMergeUs + kMergePartUs * (static_cast<float>(n) / red[2] - 1.f) * G / C : 0.f) +
                    kExtraGroupUs * fminf(ceilf(G / C) - 1.f, 3.f);
       if (static_cast<int64_t>(n) * H > a.max_groups) cost = 3e38f;
       if (lane == 0) {
         s_cost[wave] = cost;
-        s_l[wave] = L;
+        s_try[wave] = make_int4(L, n, np_most, piece);
       }
       __syncthreads();
       int at = 0;
-      for (int w = 1; w < kPlanWaves; ++w)
-        if (s_cost[w] < s_cost[at]) at = w;  // (ties: the larger L)
-      best = s_l[at];
-      hi = s_l[max(at - 1, 0)];
-      lo = s_l[min(at + 1, kPlanWaves - 1)];
+      float least_cost = s_cost[0];
+#pragma unroll
+      for (int w = 1; w < kPlanWaves; ++w) {
+        const float c = s_cost[w];
+        at = c < least_cost ? w : at;  // (ties: the larger L)
+        least_cost = fminf(c, least_cost);
+      }
+      const int4 x = s_try[at];
+      best = x.x;
+      groups = x.y * H;
+      parts = x.z;
+      longest = x.w;
+      hi = s_try[max(at - 1, 0)].x;
+      lo = s_try[min(at + 1, kPlanWaves - 1)].x;
       __syncthreads();
     }
   }
-  // ---- the groups, in sequence order; up to 3 C of them (and what LDS holds)
-  // are dealt: by size, largest first, in snake order over the CUs, on which
-  // group i and group i + C run
+  // ---- the groups, in sequence order, 1024 sequences at a time; up to 3 C of
+  // them (and what LDS holds) are dealt: by size, largest first, in snake order
+  // over the CUs, on which group i and group i + C run
   const bool dealt = groups <= min(3 * C, kPlanDealt);
-  for (int b0 = 0; b0 < a.num_seqs; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    const int64_t kv = b < a.num_seqs ? int_at(a.kv_len, a.kv_i64, b) : 0;
-    const int t = b < a.num_seqs ? planned_tiles(a, kv) : 0;
-    const int np = (t + best - 1) / best;
-    int incl = np;  // pieces up to and with sequence b
+  int4* const work = reinterpret_cast<int4*>(a.work);
+  for (int b0 = 0, base = 0; b0 < a.num_seqs; b0 += kPlanThreads) {
+    const int nb = min(kPlanThreads, a.num_seqs - b0);
+    const uint32_t mine = tid < nb ? tiles(b0 + tid) : 0;
+    const int np = static_cast<int>((mine + best - 1) / static_cast<uint32_t>(best));
+    const int incl = wave_scan(np, lane);  // pieces up to and with this sequence
+    if (lane == 63) s_red[0][wave] = incl;
+    __syncthreads();
+    int before = 0, all = 0;
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int y = __shfl_up(incl, s);
-      if (lane >= s) incl += y;
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const int x = s_red[0][w];
+      before += w < wave ? x : 0;
+      all += x;
     }
-    if (lane == 63) s_a[wave] = incl;
+    s_first[tid] = before + incl - np;
     __syncthreads();
-    int before = s_base;
-    for (int w = 0; w < wave; ++w) before += s_a[w];
-    const int first = before + incl - np;
-    for (int j = 0; j < np; ++j) {
-      const int q = t / np, r = t - q * np;
-      for (int h = 0; h < H; ++h) {
-        const int i = (first + j) * H + h;
-        if (dealt) {
-          s_size[i] = q + (j < r);
-          s_item[i] = make_int4(b, j, np, h);
-        } else {
-          const int start = j * q + min(j, r);
-          int4* e = reinterpret_cast<int4*>(a.work) + 2 * static_cast<int64_t>(i);
-          e[0] = make_int4(b, h, j, np);
-          e[1] = make_int4(start * kTile, static_cast<int>(min(kv, static_cast<int64_t>(start + q + (j < r)) * kTile)), 0, 0);
-        }
-      }
+    for (int i = tid; i < all * H; i += kPlanThreads) {
+      const int p = static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(H)), h = i - p * H;
+      int at = 0;  // the last sequence whose first piece is p or before
+#pragma unroll
+      for (int s = kPlanThreads / 2; s >= 1; s >>= 1)
+        if (at + s < nb && s_first[at + s] <= p) at += s;
+      const int b = b0 + at, j = p - s_first[at];
+      const uint32_t t = tiles(b), m = (t + best - 1) / static_cast<uint32_t>(best);
+      const int q = static_cast<int>(t / m), r = static_cast<int>(t - q * m);
+      const int start = j * q + min(j, r), size = q + (j < r);
+      const int64_t kv = int_at(a.kv_len, a.kv_i64, b);
+      const int4 e0 = make_int4(b, h, j, static_cast<int>(m));
+      const int4 e1 = make_int4(start * kTile, static_cast<int>(min(kv, static_cast<int64_t>(start + size) * kTile)), 0, 0);
+      int4* const e = dealt ? s_item : work;
+      e[2 * (static_cast<int64_t>(base) * H + i)] = e0;
+      e[2 * (static_cast<int64_t>(base) * H + i) + 1] = e1;
     }
-    __syncthreads();
-    if (tid == kPlanThreads - 1) s_base = before + incl;
+    base += all;
     __syncthreads();
   }
-  if (dealt && tid < groups) {
-    const int mine = s_size[tid];
-    int rank = 0;
-    for (int i = 0; i < groups; ++i) rank += s_size[i] > mine || (s_size[i] == mine && i < tid);
-    const int round = rank / C, pos = rank - round * C;
-    const int in_round = min(C, groups - round * C);
-    const int slot = round * C + ((round & 1) ? in_round - 1 - pos : pos);
-    const int4 it = s_item[tid];
-    const int64_t kv = int_at(a.kv_len, a.kv_i64, it.x);
-    const int t = planned_tiles(a, kv), q = t / it.z, r = t - q * it.z;
-    const int start = it.y * q + min(it.y, r);
-    int4* e = reinterpret_cast<int4*>(a.work) + 2 * static_cast<int64_t>(slot);
-    e[0] = make_int4(it.x, it.w, it.y, it.z);
-    e[1] = make_int4(start * kTile, static_cast<int>(min(kv, static_cast<int64_t>(start + mine) * kTile)), 0, 0);
+  if (dealt) {
+    // ranks by counting: a place for every size of up to 1023 tiles (larger ones
+    // share them); which of two equal groups comes first is of no consequence
+    const float step = longest < kPlanThreads ? 1.f : static_cast<float>(kPlanThreads - 1) / longest;
+    s_first[tid] = 0;
+    __syncthreads();
+    int4 e0, e1;
+    int place = 0, in_place = 0;
+    if (tid < groups) {
+      e0 = s_item[2 * tid];
+      e1 = s_item[2 * tid + 1];
+      const int size = (e1.y - e1.x + kTile - 1) / kTile;
+      place = kPlanThreads - 1 - min(kPlanThreads - 1, static_cast<int>(size * step));
+      in_place = atomicAdd(&s_first[place], 1);
+    }
+    __syncthreads();
+    const int n = s_first[tid], incl = wave_scan(n, lane);
+    if (lane == 63) s_red[0][wave] = incl;
+    __syncthreads();
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) before += w < wave ? s_red[0][w] : 0;
+    s_first[tid] = before + incl - n;
+    __syncthreads();
+    if (tid < groups) {
+      const int rank = s_first[place] + in_place;
+      const int round = static_cast<int>(static_cast<uint32_t>(rank) / static_cast<uint32_t>(C)), pos = rank - round * C;
+      const int in_round = min(C, groups - round * C);
+      const int slot = round * C + ((round & 1) ? in_round - 1 - pos : pos);
+      work[2 * slot] = e0;
+      work[2 * slot + 1] = e1;
+    }
   }
   if (a.fixed)
     for (int64_t i = groups + tid; i < a.work_cap; i += kPlanThreads)
       reinterpret_cast<int4*>(a.work)[2 * i] = make_int4(-1, 0, 0, 0);
   if (tid == 0) {
     a.status[MV_PLAN_NUM_ITEMS] = groups;
-    a.status[MV_PLAN_BAD_KV_LEN] = s_bad;
-    a.status[MV_PLAN_INSUFFICIENT] = s_short;
+    a.status[MV_PLAN_BAD_KV_LEN] = red[3];
+    a.status[MV_PLAN_INSUFFICIENT] = red[4];
     a.status[MV_PLAN_BAD_BLOCK] = 0;
     a.status[MV_PLAN_MAX_PARTS] = parts;
-    a.status[MV_PLAN_MIN_KV_LEN] = s_min;
+    a.status[MV_PLAN_MIN_KV_LEN] = a.num_seqs ? -red[5] : INT_MAX;
     a.status[MV_PLAN_PARTITION_TOKENS] = longest * kTile;
     a.status[MV_PLAN_IDS_PER_ITEM] =
         ids_stride(a.fixed ? static_cast<int64_t>(a.max_blocks) << a.bs_log2 : static_cast<int64_t>(longest) * kTile, a.bs_log2);
@@ -638,7 +693,7 @@ __global__ __launch_bounds__(256) void fp8_decode_ids_kernel(Fp8DecodePlanArgs a
     ids[i] = ok ? static_cast<int32_t>(blk) : -1;
     bad += !ok && e0.y == 0 && ((first + i) << a.bs_log2) >= e1.x;
   }
-  bad = wave_sum(bad);
+  bad = wave_reduce(bad, Sum());
   if (bad && lane == 0) atomicAdd(&a.status[MV_PLAN_BAD_BLOCK], bad);
 }
 
