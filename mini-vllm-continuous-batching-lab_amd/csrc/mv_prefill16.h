@@ -102,8 +102,11 @@ __device__ __forceinline__ float halves_sum(float x) {
 // to an area of their own), and converted in place. Chunk keys are copied as in
 // the kernel of a 16-bit pool. HALF: a wave copies K (v false) or V only. Measured
 // (us, 4 x (1536 + 512) at 14 / 2 x 64; 8 x (300-2900 + 100-900) at 28 / 4 x 128):
-// all in place 30.6 and 133; as it is 29.3 and 125, where a 16-bit pool takes
-// 24.5 and 116. Without the conversion and its LDS stores it is 27.5 and 117.
+// all in place 30.6 and 133; as it is 27.3 and 126, where a 16-bit pool takes 24.2
+// and 117. What is left is issue slots: two waves of a SIMD share them, and the
+// conversion (16 instructions for 1 KB of codes), its stores and the branches
+// that tell prefix from chunk stages all take some. Writing the rows half a stage
+// earlier, out of the way of the barrier, was no faster (30.4 against 29.4).
 template <int DTYPE, int D, bool HALF>
 struct Fp8SubTile {
   using B = SubTileCopy<DTYPE, D>;
@@ -112,13 +115,15 @@ struct Fp8SubTile {
   static constexpr bool kRegs = D == 64 || HALF;
   u32x4 codes[kRegs ? NT : 1][kRegs ? CL : 1];
   float scale[NT];
-  int rows;  // prefix rows of the sub-tile in flight
+  int rows;  // prefix rows of the sub-tile that settles
 
   // Starts the loads of the codes of the sub-tile that begins with key kb; their
   // LDS address dst and the mixed sub-tile's are of no use with kRegs.
   __device__ __forceinline__ void fetch(const B& copy, int kb, uint32_t dst, uint32_t mix, int block_id, bool v) {
-    rows = min(max(copy.cached - kb, 0), kTile);
-    if (rows == 0) return;
+    if constexpr (!kRegs) {  // (with kRegs the caller counts the stages that have codes)
+      rows = min(max(copy.cached - kb, 0), kTile);
+      if (rows == 0) return;
+    }
     const PrefillArgs& a = copy.a;
     const uint32_t code_dst = rows < kTile ? mix : dst;
     const int code_step = rows < kTile ? kCodeBytes : B::G::kTileBytes;
@@ -160,6 +165,7 @@ struct Fp8SubTile {
   // returns the loads of which no row is to be cleared.
   __device__ __forceinline__ unsigned copy_rows(const B& copy, int kb, int win_blk0, uint32_t dst, int block_id,
                                                 bool v) const {
+    const int rows = min(max(copy.cached - kb, 0), kTile);
     if (rows == 0) {
       if constexpr (HALF) {
         if (v) return copy.template copy<false, true>(kb, win_blk0, dst, block_id);
@@ -193,7 +199,7 @@ struct Fp8SubTile {
 
   // Turns the landed codes into their rows of the sub-tile at s_sub.
   __device__ __forceinline__ void settle(char* s_sub, const char* s_mix, int lane, bool v) const {
-    if (rows == 0) return;
+    if (!kRegs && rows == 0) return;
     asm volatile("" : "+v"(lane));  // (these addresses are not kept through the key loop)
     const int row = lane >> 2, piece = (lane & 3) * 2, sw = piece_swizzle<8>(row);
 #pragma unroll
@@ -384,22 +390,32 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
       return copy.copy(kb, win_blk0, dst, id);
     }
   };
-  // The codes of stage k into registers (kCodeRegs): free once a stage landed.
+  // kCodeRegs: the window's stages whose sub-tile of this wave has codes, and those
+  // that have nothing else, counted here, not in the key loop (4 prompts of 2048
+  // tokens at 14 / 2 x 64: 47.3 -> 46.1 us; 16 x (1536 + 512) 83.9 -> 81.6); the
+  // first sub-tile's distance to the prefix's end.
+  [[maybe_unused]] int n_codes = 0, n_only = 0, lead = 0;
+  const bool half_v = Tr::kHalfSubs && (wave & 1);
+  // The codes of stage k into registers: free once a stage landed.
   auto fetch_codes = [&](int k, int id) __attribute__((always_inline)) {
-    if constexpr (kCodeRegs) fp8.fetch(copy, k * Tr::kStageTokens + su * kTile, 0, 0, id, Tr::kHalfSubs && (wave & 1));
+    if constexpr (kCodeRegs) fp8.fetch(copy, k * Tr::kStageTokens + su * kTile, 0, 0, id, half_v);
   };
   // Waits for this wave's copies of a stage (the next stage's may stay in
   // flight) and meets the other waves: the stage is whole, and every wave has
   // read what it needs of the one before. V slots of keys that were not
   // loaded read pool row 0 instead: they are cleared first (P is 0 there, but
-  // 0 * NaN would not be). next_codes: 8-bit codes, loads those of the stage after.
-  auto land = [&](int st, unsigned ok, bool more, auto next_codes) __attribute__((always_inline)) {
+  // 0 * NaN would not be). 8-bit codes: those of the stage (i of the window) become
+  // rows, next_codes loads those of the stage after.
+  auto land = [&](int i, int st, unsigned ok, bool more, auto next_codes) __attribute__((always_inline)) {
     if constexpr (Tr::kFp8) wait_vmcnt<0>();  // (one stage in flight)
     else wait_vmcnt_groups<Tr::kWaveLoads, 1>(more);
     asm volatile("" ::: "memory");
-    if constexpr (Tr::kFp8)
-      fp8.settle(s_lds + st * Tr::kStageBytes + su * Tr::kSubBytes, s_lds + Tr::kMixOffset, lane,
-                 Tr::kHalfSubs && (wave & 1));
+    if constexpr (Tr::kFp8) {
+      if (!kCodeRegs || i < n_codes) {
+        if constexpr (kCodeRegs) fp8.rows = min(kTile, lead - i * Tr::kStageTokens);
+        fp8.settle(s_lds + st * Tr::kStageBytes + su * Tr::kSubBytes, s_lds + Tr::kMixOffset, lane, half_v);
+      }
+    }
     next_codes();
     if (__builtin_amdgcn_ballot_w64(ok != copy.kAllValid) != 0) {
       char* vdst = s_lds + st * Tr::kStageBytes + su * Tr::kSubBytes + Tr::kTileBytes;
@@ -477,11 +493,16 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
     __syncthreads();  // block ids of the window visible; previous window's stages released
     const int k0 = first / Tr::kStageTokens;
     const int ns = (min(key_end, win0 + win_tokens) - first + Tr::kStageTokens - 1) / Tr::kStageTokens;
-    fetch_codes(k0, stage_id(k0));
+    if constexpr (kCodeRegs) {
+      lead = cached - (k0 * Tr::kStageTokens + su * kTile);
+      n_codes = min(ns, (max(lead, 0) + Tr::kStageTokens - 1) / Tr::kStageTokens);
+      n_only = min(ns, (max(lead - kTile, -Tr::kStageTokens) + Tr::kStageTokens) / Tr::kStageTokens);
+      if (n_codes > 0) fetch_codes(k0, stage_id(k0));
+    }
     const unsigned ok = issue(k0, 0, stage_id(k0));
     unsigned ok_next = 0;
     if (!Tr::kFp8 && ns > 1) ok_next = issue(k0 + 1, 1, stage_id(k0 + 1));
-    land(0, ok, ns > 1, [&] { if (ns > 1) fetch_codes(k0 + 1, stage_id(k0 + 1)); });
+    land(0, 0, ok, ns > 1, [&] { if (1 < n_codes) fetch_codes(k0 + 1, stage_id(k0 + 1)); });
     if (Tr::kFp8 && ns > 1) ok_next = issue(k0 + 1, 1, stage_id(k0 + 1));
 
     // this wave's tiles that some row of it sees, and the stages full of them
@@ -501,14 +522,16 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
       auto step = [&](auto st_c) __attribute__((always_inline)) {
         constexpr int ST = decltype(st_c)::value;
         [[maybe_unused]] int code_id = 0;
-        if constexpr (kCodeRegs) code_id = stage_id(k0 + i + 2);
+        if (kCodeRegs && i + 2 < n_codes) code_id = stage_id(k0 + i + 2);
         do_tile(set_key + i * T * SETS * 32, s[0], IntC<1>{}, s[1], [&] { read_k(ST, kTileStep); });
         read_v(ST, kTileStep);
-        if (i + 1 < ns) land(ST ^ 1, ok_next, false, [&] { if (i + 2 < ns) fetch_codes(k0 + i + 2, code_id); });
-        const int id = stage_id(k0 + i + 2);
+        if (i + 1 < ns)
+          land(i + 1, ST ^ 1, ok_next, false, [&] { if (i + 2 < n_codes) fetch_codes(k0 + i + 2, code_id); });
+        const int id = kCodeRegs ? 0 : stage_id(k0 + i + 2);  // (no copies from the pool)
         do_tile(set_key + (i * T + 1) * SETS * 32, s[1], IntC<1>{}, s[0], [&] { read_k(ST ^ 1, 0); });
         read_v(ST ^ 1, 0);
-        if (i + 2 < ns) ok_next = issue(k0 + i + 2, ST, id);
+        if (kCodeRegs && i + 2 < n_only) ok_next = copy.kAllValid;
+        else if (i + 2 < ns) ok_next = issue(k0 + i + 2, ST, id);
         asm volatile("" ::: "memory");
         ++i;
       };
@@ -530,7 +553,7 @@ __device__ __forceinline__ void prefill16(const PrefillArgs& a) {
         do_tile(set_key + (i * T + t) * SETS * 32, s, IntC<0>{}, s, [] {});
       }
       if (i + 1 < ns)
-        land(st ^ 1, ok_next, false, [&] { if (i + 2 < ns) fetch_codes(k0 + i + 2, stage_id(k0 + i + 2)); });
+        land(i + 1, st ^ 1, ok_next, false, [&] { if (i + 2 < n_codes) fetch_codes(k0 + i + 2, stage_id(k0 + i + 2)); });
       if (i + 2 < ns) ok_next = issue(k0 + i + 2, st, stage_id(k0 + i + 2));
       asm volatile("" ::: "memory");
     }
