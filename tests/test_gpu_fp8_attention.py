@@ -232,6 +232,31 @@ def test_prefill(i):
     assert torch.equal(bits(out), bits(again))
 
 
+@pytest.mark.parametrize("bs,hq,hkv,d,new", [(16, 14, 2, 64, 2), (16, 14, 2, 64, 37), (32, 7, 1, 128, 2),
+                                             (64, 14, 2, 128, 37)])
+def test_prefill_every_prefix_end(bs, hq, hkv, d, new):
+    """Prefixes that end at every place of two stages of keys: the bits of the 16-bit
+    kernel over the values the codes stand for, few sequences at a time and all at once."""
+    dtype = torch.bfloat16
+    cached = list(range(0, 260, 1 if new == 2 else 3))
+    table, num_blocks = _tables(cached, bs, d)
+    kc, vc, sc = fp8_util.random_pool(num_blocks, hkv, bs, d, new, DEV)
+    _poison(kc, vc, table, cached, bs)
+    pool = [(c.float() * sc[:, :, j, None, None]).to(dtype) for j, c in enumerate((kc, vc))]
+    g = torch.Generator().manual_seed(d + new)
+    t = len(cached) * new
+    q = torch.randn(t, hq, d, generator=g).to(dtype).to(DEV)
+    k, v = (torch.randn(t, hkv, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    table = table.to(DEV)
+    for first, count in ((0, len(cached)), (5, 40), (60, 25)):
+        rows, lens = list(range(first, first + count)), cached[first:first + count]
+        part = slice(first * new, (first + count) * new)
+        got = fp8.hip_fp8_prefill_attention(q[part], k[part], v[part], kc, vc, sc, table, rows, lens,
+                                            [new] * count, bs)
+        want = gpu.hip_prefill_attention(q[part], k[part], v[part], *pool, table, rows, lens, [new] * count, bs)
+        assert not torch.isnan(got).any() and torch.equal(bits(got), bits(want)), (first, count)
+
+
 def test_prefill_errors():
     table, num_blocks, kc, vc, sc, q, k, v = _prefill_inputs(1)
     seqs, bs, hq, hkv, d, dtype = PREFILL[1]
