@@ -704,6 +704,7 @@ int mv_fp8_write_plan(const int64_t* slot_mapping, int64_t num_tokens, int32_t b
  *   grows, the block's other rows are scaled to it, rounded to nearest even.
  * items, table, plan_status: mv_fp8_write_plan's, over the same num_tokens;
  * max_items bounds the items it may have found (num_tokens if not known).
+ * query_out may be query; key_out must not overlap key or value.
  */
 int mv_fp8_kv_cache_write(
     const void* query, int64_t q_stride_tok, int64_t q_stride_head, void* query_out,

@@ -604,6 +604,9 @@ extern "C" int mv_fp8_kv_cache_write(
     return fail(MV_ERR_INVALID_ARGUMENT,
                 "mv_fp8_kv_cache_write: rotation needs positions, both tables and the query's rows; without it "
                 "there is no query and no key_out");
+  // (the rows' groups and the cache's read the key at the same time)
+  if (key_out && (key_out == key || key_out == value))
+    return fail(MV_ERR_INVALID_ARGUMENT, "mv_fp8_kv_cache_write: key_out must not be the key's or the value's rows");
   const void* ptrs[] = {query, query_out, key, key_out, value, key_cache, value_cache, cos_table, sin_table};
   for (const void* p : ptrs)
     if (p && off16(p))

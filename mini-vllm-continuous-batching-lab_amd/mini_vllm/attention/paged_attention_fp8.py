@@ -23,7 +23,8 @@ fp16 or bf16, ``block_size`` a power of two from 16 to 256, ``head_dim`` 64 or
 128; anything else is refused.
 
 Plans. What the layers of a step share (the tokens' blocks, the work lists) is
-planned once, checked on the device and read back (one synchronisation):
+planned once, checked on the device and read back (one synchronisation); the
+plan keeps no reference to the metadata, which may change afterwards:
 ``plan_fp8_write``, ``plan_fp8_decode``, ``plan_fp8_prefill``,
 ``plan_fp8_gather``. The entry points take such a plan as ``plan``, made from the
 same metadata; without one they make it, and find it again for the step's other
@@ -200,6 +201,8 @@ def plan_fp8_write(
         capture = _gpu._capture_id(device)
         slots = _i64(slot_mapping, device)
         pos = None if positions is None else _i64(positions, device)
+        if pos is positions and pos is not None and not capture:
+            pos = pos.clone()  # (the plan's own: the calls read it)
         ws_bytes = lib.mv_fp8_write_plan_workspace_bytes(n)
         # status, items, table and the hash table of large steps in one buffer
         words = _hip.MV_FP8_PLAN_WORDS + n
@@ -658,6 +661,8 @@ def plan_fp8_prefill(
                                "(hip_fp8_prefill_attention plans on the device there)")
         cached, qlens = _gpu._host_lengths(cached_len_before, query_len)
         assert len(rows) == len(cached) == len(qlens)
+        if block_table.device == device:
+            block_table = block_table.clone()  # (the plan's own: the calls read it)
         made = _gpu._prefill_plan_make(block_table, rows, cached, qlens, block_size, num_blocks,
                                        num_q_heads, num_kv_heads, head_dim, dtype, device)
         bt, meta, work, ws = made[0], made[1], made[2], made[7]

@@ -105,6 +105,14 @@ def test_refused(lib, name, change, code):
     assert name.encode() in lib.mv_last_error() or b"mv_paged_prefill" in lib.mv_last_error()
 
 
+def test_key_out_is_no_input(lib):
+    """The append reads the key in two places at once: it is not rotated in place."""
+    for change in (dict(ko=BUF), dict(ko=2 * BUF, v=2 * BUF)):
+        args = dict(WRITE, **change)
+        assert getattr(lib, "mv_fp8_kv_cache_write")(*args.values()) == INVALID
+        assert b"key_out must not" in lib.mv_last_error()
+
+
 def test_nothing_to_do(lib):
     assert lib.mv_fp8_kv_cache_write(*{**WRITE, "n": 0}.values()) == 0
     assert lib.mv_fp8_paged_decode(*{**DECODE, "groups": 0}.values()) == 0

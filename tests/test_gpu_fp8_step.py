@@ -456,3 +456,69 @@ def test_pools_past_4_gib():
         del kc, vc, sc
     for x, y in zip(*got):
         assert torch.equal(x, y)
+
+
+def test_a_plan_keeps_its_own_metadata():
+    """Metadata tensors that change after an eager plan was made do not change its calls."""
+    hq, hkv, d, bs, dtype, nb = 14, 2, 64, 16, torch.bfloat16, 8
+    rope = _rope(d, dtype, 64)
+    kc, vc, sc = fp8_util.random_pool(nb, hkv, bs, d, 1, DEV)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(3, hq, d, generator=g).to(dtype).to(DEV)
+    k, v = (torch.randn(3, hkv, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+    slots, positions = torch.tensor([40, 41, 42], device=DEV), torch.tensor([8, 9, 10], device=DEV)
+    table, kv = torch.tensor([[2, 5]], device=DEV), torch.tensor([27], device=DEV)
+    plans = (fp8.plan_fp8_write(slots, bs, nb, DEV, positions, 64),
+             fp8.plan_fp8_decode(table, kv, bs, nb, DEV, d, hkv),
+             fp8.plan_fp8_prefill(table, [0], [24], [3], bs, nb, hq, hkv, d, dtype, DEV),
+             fp8.plan_fp8_gather(table, [27], [0], bs, nb, DEV))
+
+    def run(write=None, decode=None, prefill=None, gather=None):
+        pool = [x.clone() for x in (kc, vc, sc)]
+        qr, kr = fp8.hip_fp8_rope_kv_cache_write(q, k, v, positions, rope.cos, rope.sin, *pool, slots, bs,
+                                                 plan=write)
+        return [pool[0].view(torch.uint8), pool[1].view(torch.uint8), pool[2], qr, kr,
+                fp8.hip_fp8_decode_attention(q[:1], *pool, table, kv, bs, plan=decode),
+                fp8.hip_fp8_prefill_attention(qr, kr, v, *pool, table, [0], [24], [3], bs, plan=prefill),
+                *fp8.gather_fp8_prefix_kv(*pool, table, [27], [0], bs, dtype, plan=gather)]
+
+    want = run()
+    for t, x in ((slots, [7, 8, 9]), (positions, [60, 61, 62]), (table, [[6, 7]]), (kv, [3])):
+        t.copy_(torch.tensor(x))
+    got = run(*plans)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("t", [70, 3000])
+def test_captured_append_of_a_prompt(t):
+    """An append captured once (its plan in one launch or four), replayed with other
+    slots and rows, eager work between the replays."""
+    hkv, d, bs, dtype, nb = 2, 64, 32, torch.bfloat16, 128
+    g = torch.Generator().manual_seed(t)
+    kc, vc, sc = fp8_util.random_pool(nb, hkv, bs, d, 1, DEV)
+    slots = torch.arange(t, device=DEV) + 5
+    k, v = (torch.empty(t, hkv, d, dtype=dtype, device=DEV) for _ in range(2))
+
+    def fill():
+        for x in (k, v):
+            x.copy_(torch.randn(x.shape, generator=g) * 3)
+
+    fill()
+    own = [x.clone() for x in (kc, vc, sc)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fp8.hip_fp8_cache_write(k, v, kc, vc, sc, slots, bs)
+    gid = gpu.last_capture_id()
+    for n in range(4):
+        fill()
+        order = torch.randperm(nb * bs, generator=g)[:t] if n % 2 else torch.arange(t) + 32 * n + n
+        slots.copy_(order)
+        slots[t // 2] = -1
+        graph.replay()
+        gpu.check_deferred(gid)
+        fp8.hip_fp8_cache_write(k, v, *own, slots.clone(), bs)
+        torch.cuda.synchronize()
+        for a, b in zip((kc, vc), own):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert torch.equal(sc, own[2])
+    gpu.clear_deferred(gid)
