@@ -102,8 +102,8 @@ __device__ __forceinline__ float halves_sum(float x) {
 // to an area of their own), and converted in place. Chunk keys are copied as in
 // the kernel of a 16-bit pool. HALF: a wave copies K (v false) or V only. Measured
 // (us, 4 x (1536 + 512) at 14 / 2 x 64; 8 x (300-2900 + 100-900) at 28 / 4 x 128):
-// all in place 30.6 and 133; as it is 27.3 and 126, where a 16-bit pool takes 24.2
-// and 117. What is left is issue slots: two waves of a SIMD share them, and the
+// all in place 30.6 and 133; as it is 26.9 and 124, where a 16-bit pool takes 24.3
+// and 116. What is left is issue slots: two waves of a SIMD share them, and the
 // conversion (16 instructions for 1 KB of codes), its stores and the branches
 // that tell prefix from chunk stages all take some. Writing the rows half a stage
 // earlier, out of the way of the barrier, was no faster (30.4 against 29.4).
@@ -113,6 +113,10 @@ struct Fp8SubTile {
   static constexpr int CL = D / 64, NT = HALF ? 1 : 2;
   static constexpr int kCodeBytes = kTile * D;
   static constexpr bool kRegs = D == 64 || HALF;
+  // lane addresses are kept through the key loop only where that is faster: 128 rows
+  // at head_dim 64 (27.5 -> 26.9); with 256 rows chunk stages lose by it (46.3 ->
+  // 47.2, 4 prompts of 2048), at head_dim 128 there are no registers
+  static constexpr bool kOpaque = D == 128 || HALF;
   u32x4 codes[kRegs ? NT : 1][kRegs ? CL : 1];
   float scale[NT];
   int rows;  // prefix rows of the sub-tile that settles
@@ -134,7 +138,7 @@ struct Fp8SubTile {
     // lane l of load c: row l / 4, 16 dims from 64 c + 16 (l % 4) (the 16-bit rows'
     // stores then fall into different banks)
     int lane = copy.lane;
-    asm volatile("" : "+v"(lane));
+    if constexpr (kOpaque) asm volatile("" : "+v"(lane));
     const uint32_t lane_off = (lane >> 2) * D + (lane & 3) * 16;
     // (vector loads of the scales: a scalar load in flight would turn every LDS
     // wait until its use into one for it)
@@ -200,7 +204,7 @@ struct Fp8SubTile {
   // Turns the landed codes into their rows of the sub-tile at s_sub.
   __device__ __forceinline__ void settle(char* s_sub, const char* s_mix, int lane, bool v) const {
     if (!kRegs && rows == 0) return;
-    asm volatile("" : "+v"(lane));  // (these addresses are not kept through the key loop)
+    if constexpr (kOpaque) asm volatile("" : "+v"(lane));
     const int row = lane >> 2, piece = (lane & 3) * 2, sw = piece_swizzle<8>(row);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
