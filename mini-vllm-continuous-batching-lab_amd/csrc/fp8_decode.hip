@@ -136,7 +136,8 @@ __global__ __launch_bounds__(kDwWaves * 64) __attribute__((amdgpu_waves_per_eu(2
     // an id outside the pool is never an address: its tiles read block 0 and
     // are masked
     const bool have = static_cast<uint32_t>(id) < a.num_blocks;
-    const uint64_t have_mask = __builtin_amdgcn_ballot_w64(have);
+    // (lanes past the wave's tiles count as held: what they read is no id)
+    const uint64_t have_mask = __builtin_amdgcn_ballot_w64(have || lane >= nw);
     const int64_t bh = static_cast<int64_t>(have ? id : 0) * a.num_kv_heads + h;
     const float2 s2 = reinterpret_cast<const float2*>(a.scales)[bh];
     // this lane's tile's place in the pools, in bytes
