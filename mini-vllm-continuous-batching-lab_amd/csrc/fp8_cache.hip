@@ -480,7 +480,9 @@ struct Fp8GatherArgs {
   int32_t num_kv_heads, bs_log2;
 };
 
-// out[t, h, :] = codes * scale; 16 codes a thread, rows outside the pool 0.
+// out[t, h, :] = codes * scale; 16 codes a thread, rows outside the pool 0. Bound:
+// its writes, twice the bytes read; 61152 tokens of 4 x 128 35.5 us (188 MB, 5.3
+// TB/s, a large copy's rate), 301 tokens of 2 x 64 2.2 (a launch).
 template <int DTYPE, int D>
 __global__ __launch_bounds__(256) void fp8_gather_kernel(Fp8GatherArgs a) {
   constexpr int kPer = D / 16;

@@ -24,6 +24,12 @@
 // The scaled conversions make 16-bit operands of the codes, exactly.
 // Softmax: one pass; a head's reference m moves (and O and l are rescaled)
 // only where a lane's sum of p = exp2(s - m) would pass 4096.
+// Measured (us a call, codes from HBM): 1 x 701 tokens at 14 / 2 x 64 5.3, 64 x
+// 128-2048 9.3, 16 x 8k-32k 18.7 (4.3 TB/s), 128 x 512-4096 at 28 / 4 x 128 52.2 (6.0
+// TB/s; 62.7 with pointer loads and accumulators in AGPRs, which were copied for
+// every pair of tiles: two waves per SIMD are asked for, so that they stay in
+// VGPRs). 8 or 16 waves a group and 3 or 4 pairs of tiles in flight gained nothing:
+// a CU streams 40 KB per us either way.
 #include <algorithm>
 #include <climits>
 

@@ -1,7 +1,9 @@
 // Prefill attention over the 8-bit KV cache (format: mv_fp8.h): the 16-bit
 // kernels (mv_prefill16.h) with the prefix's codes turned into 16-bit values on
 // their way into LDS. What a code stands for is a number of the model's type, so
-// the result is the 16-bit kernel's over the dequantised pool, bit for bit.
+// the result is the 16-bit kernel's over the dequantised pool, bit for bit. Bound
+// as there, by issue slots beside the MFMAs; the conversion takes 5-11 % (measured
+// beside Fp8SubTile): 8 x (300-2900 + 100-900) at 28 / 4 x 128 124 us, 844 TFLOP/s.
 #include "mv_prefill16.h"
 
 namespace mv {
