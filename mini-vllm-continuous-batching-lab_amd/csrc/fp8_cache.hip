@@ -214,29 +214,46 @@ __device__ __forceinline__ void rotate_pair(const uint4 x1, const uint4 x2, cons
   y2 = rotate_chunk<DTYPE>(x2, x1, c2, s2, false);
 }
 
-// The query rows (and with k_out the key rows), rotated: a thread owns 8
-// pairs (d, d + D/2) of one (token, head).
+// The query rows (and with k_out the key rows), rotated: a thread owns 8 pairs
+// (d, d + D/2) of two heads of a token, which share the tables' values. (9 k
+// tokens at 28 / 4 x 128, outputs not in a cache: 38.5 us with one head a thread,
+// 36.4 with two, 36.9 with four. Non-temporal stores take another 2 off, and
+// give it back in the attention that reads the rows next.)
+constexpr int kRotHeads = 2;
+
 template <int DTYPE, int D>
 __device__ __forceinline__ void rotate_rows(const Fp8WriteArgs& a, int group, int groups) {
   constexpr int kPer = D / 16;
   const int heads = a.num_q_heads + (a.k_out ? a.num_kv_heads : 0);
-  const int64_t total = static_cast<int64_t>(a.num_tokens) * heads * kPer;
+  const int sets = (heads + kRotHeads - 1) / kRotHeads;
+  const int64_t total = static_cast<int64_t>(a.num_tokens) * sets * kPer;
   for (int64_t i = static_cast<int64_t>(group) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(groups) * 256) {
     const int c = static_cast<int>(i % kPer);
-    const int64_t th = i / kPer;
-    const int hh = static_cast<int>(th % heads);
-    const int64_t t = th / heads;
-    const bool is_q = hh < a.num_q_heads;
-    const int h = is_q ? hh : hh - a.num_q_heads;
-    const char* x = is_q ? a.q + t * a.q_st + h * a.q_sh : a.k + t * a.k_st + h * a.k_sh;
-    char* y = is_q ? a.q_out + t * a.qo_st + h * a.qo_sh : a.k_out + t * a.ko_st + h * a.ko_sh;
+    const int64_t ts = i / kPer;
+    const int64_t t = ts / sets;
+    const int h0 = static_cast<int>(ts - t * sets) * kRotHeads;
     const int64_t row = clamped_position<DTYPE>(a, t) * a.table_stride;
     const int o1 = c * 16, o2 = o1 + D;
-    uint4 y1, y2;
-    rotate_pair<DTYPE>(*reinterpret_cast<const uint4*>(x + o1), *reinterpret_cast<const uint4*>(x + o2),
-                       a.cos + row, a.sin + row, o1, o2, y1, y2);
-    *reinterpret_cast<uint4*>(y + o1) = y1;
-    *reinterpret_cast<uint4*>(y + o2) = y2;
+    const uint4 c1 = *reinterpret_cast<const uint4*>(a.cos + row + o1), c2 = *reinterpret_cast<const uint4*>(a.cos + row + o2);
+    const uint4 s1 = *reinterpret_cast<const uint4*>(a.sin + row + o1), s2 = *reinterpret_cast<const uint4*>(a.sin + row + o2);
+    uint4 x1[kRotHeads], x2[kRotHeads];
+    char* y[kRotHeads];
+#pragma unroll
+    for (int k = 0; k < kRotHeads; ++k) {
+      const int hh = min(h0 + k, heads - 1);
+      const bool is_q = hh < a.num_q_heads;
+      const int h = is_q ? hh : hh - a.num_q_heads;
+      const char* x = is_q ? a.q + t * a.q_st + h * a.q_sh : a.k + t * a.k_st + h * a.k_sh;
+      y[k] = is_q ? a.q_out + t * a.qo_st + h * a.qo_sh : a.k_out + t * a.ko_st + h * a.ko_sh;
+      x1[k] = *reinterpret_cast<const uint4*>(x + o1);
+      x2[k] = *reinterpret_cast<const uint4*>(x + o2);
+    }
+#pragma unroll
+    for (int k = 0; k < kRotHeads; ++k) {
+      if (h0 + k >= heads) break;
+      *reinterpret_cast<uint4*>(y[k] + o1) = rotate_chunk<DTYPE>(x1[k], x2[k], c1, s1, true);
+      *reinterpret_cast<uint4*>(y[k] + o2) = rotate_chunk<DTYPE>(x2[k], x1[k], c2, s2, false);
+    }
   }
 }
 
@@ -279,9 +296,9 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
 // dependent loads (plan words; row, position and scale; cos and sin; codes
 // that shrink): 3.0 us for one row at 14 / 2 x 64 with the query's rotation,
 // 4.2 for 64 (3.25 and 4.45 with the plan's words in two rounds and the wave's
-// maximum through LDS). A prompt's is bound by its bytes: 31.2 us for 166 MB
-// (9 k tokens at 28 / 4 x 128, rotation and returned key), 5.3 TB/s, a large
-// copy's rate.
+// maximum through LDS). A prompt's is bound by its bytes: 36.4 us for 166 MB (9 k
+// tokens at 28 / 4 x 128, rotation and returned key), 4.6 TB/s, nine tenths of a
+// large copy's rate; 30 where the outputs' memory is still in a cache.
 template <int DTYPE, int D, bool FIT>
 __device__ __forceinline__ void write_units(const Fp8WriteArgs& a) {
   constexpr int kPer = D / 16;  // threads per row
@@ -481,8 +498,11 @@ struct Fp8GatherArgs {
 };
 
 // out[t, h, :] = codes * scale; 16 codes a thread, rows outside the pool 0. Bound:
-// its writes, twice the bytes read; 61152 tokens of 4 x 128 35.5 us (188 MB, 5.3
-// TB/s, a large copy's rate), 301 tokens of 2 x 64 2.2 (a launch).
+// its writes, twice the bytes read; 61152 tokens of 4 x 128 41 us (188 MB, 4.6 TB/s,
+// nine tenths of a large copy's rate; 30-36 where the outputs' memory is still in
+// a cache), 301 tokens of 2 x 64 2.2 (a launch). 8 codes a thread 57, K and V in
+// one thread 40.7. Non-temporal stores: 37.5, but a copy of the rows right after
+// then takes 5 us more.
 template <int DTYPE, int D>
 __global__ __launch_bounds__(256) void fp8_gather_kernel(Fp8GatherArgs a) {
   constexpr int kPer = D / 16;
@@ -654,7 +674,8 @@ extern "C" int mv_fp8_kv_cache_write(
   const int unit_threads = std::min(256, block_size * head_dim / 16);
   const int64_t write = (static_cast<int64_t>(a.max_items) * num_kv_heads * 2 * unit_threads + 255) / 256;
   a.write_groups = static_cast<int>(std::min<int64_t>(write, 8192));
-  const int64_t rot = rope ? num_tokens * (num_q_heads + (key_out ? num_kv_heads : 0)) * (head_dim / 16) : 0;
+  const int64_t heads = num_q_heads + (key_out ? num_kv_heads : 0);
+  const int64_t rot = rope ? num_tokens * ((heads + kRotHeads - 1) / kRotHeads) * (head_dim / 16) : 0;
   const int groups = a.write_groups + static_cast<int>(std::min<int64_t>((rot + 255) / 256, 8192));
   if (groups == 0) return MV_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
