@@ -423,7 +423,7 @@ __global__ __launch_bounds__(kDwWaves * 64) __attribute__((amdgpu_waves_per_eu(2
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kPlanDealt = 1024;    // groups of a launch that is dealt, at most
-constexpr int kPlanSeqs = 4096;     // sequences whose tiles are kept in LDS
+constexpr int kPlanSeqs = 4096;     // sequences whose lengths are kept in LDS
 constexpr int kPlanMaxParts = 128;  // pieces of a sequence
 constexpr int kPlanMinTiles = 4;    // tiles of a piece: one for each wave
 constexpr float kHbmBytesPerUs = 6.3e6f;
@@ -489,15 +489,15 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
   return x;
 }
 
-// Tiles of sequence b that are planned: 0 where its length is below 1 or past
+// A sequence's tokens that are planned: 0 where its length is below 1 or past
 // its table row (reported).
-__device__ __forceinline__ int planned_tiles(const Fp8DecodePlanArgs& a, int64_t kv) {
-  if (kv < 1 || kv > (static_cast<int64_t>(a.max_blocks) << a.bs_log2)) return 0;
-  return static_cast<int>((kv + kTile - 1) / kTile);
+__device__ __forceinline__ int planned_tokens(const Fp8DecodePlanArgs& a, int64_t kv) {
+  return kv < 1 || kv > (static_cast<int64_t>(a.max_blocks) << a.bs_log2) ? 0 : static_cast<int>(kv);
 }
+__device__ __forceinline__ int tiles_of(int tokens) { return (tokens + kTile - 1) / kTile; }
 
 __global__ __launch_bounds__(kPlanThreads) void fp8_decode_plan_kernel(Fp8DecodePlanArgs a) {
-  __shared__ int s_tiles[kPlanSeqs];        // tiles of the first sequences
+  __shared__ int s_tokens[kPlanSeqs];       // of the first sequences
   __shared__ int s_red[6][kPlanWaves];      // totals of the waves
   __shared__ int4 s_try[kPlanWaves];        // a tried L, its groups / H, pieces, longest piece
   __shared__ float s_cost[kPlanWaves];
@@ -505,15 +505,16 @@ __global__ __launch_bounds__(kPlanThreads) void fp8_decode_plan_kernel(Fp8Decode
   __shared__ int4 s_item[2 * kPlanDealt];   // the groups to deal, as in the work list
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int H = a.num_kv_heads, C = a.cu_count;
-  auto tiles = [&](int b) {
-    return b < kPlanSeqs ? s_tiles[b] : planned_tiles(a, int_at(a.kv_len, a.kv_i64, b));
+  auto tokens = [&](int b) {
+    return b < kPlanSeqs ? s_tokens[b] : planned_tokens(a, int_at(a.kv_len, a.kv_i64, b));
   };
+  auto tiles = [&](int b) { return static_cast<uint32_t>(tiles_of(tokens(b))); };
   // ---- lengths: checks, all tiles, the most tiles of a sequence
   int red[6] = {0, 0, 0, 0, 0, -INT_MAX};  // tiles, most, sequences, too short, too long, -shortest
   for (int b = tid; b < a.num_seqs; b += kPlanThreads) {
     const int64_t kv = int_at(a.kv_len, a.kv_i64, b);
-    const int t = planned_tiles(a, kv);
-    if (b < kPlanSeqs) s_tiles[b] = t;
+    const int n = planned_tokens(a, kv), t = tiles_of(n);
+    if (b < kPlanSeqs) s_tokens[b] = n;
     red[0] += t;
     red[1] = max(red[1], t);
     red[2] += t > 0;
@@ -621,15 +622,18 @@ __global__ __launch_bounds__(kPlanThreads) void fp8_decode_plan_kernel(Fp8Decode
       for (int s = kPlanThreads / 2; s >= 1; s >>= 1)
         if (at + s < nb && s_first[at + s] <= p) at += s;
       const int b = b0 + at, j = p - s_first[at];
-      const uint32_t t = tiles(b), m = (t + best - 1) / static_cast<uint32_t>(best);
+      const int len = tokens(b);
+      const uint32_t t = tiles_of(len), m = (t + best - 1) / static_cast<uint32_t>(best);
       const int q = static_cast<int>(t / m), r = static_cast<int>(t - q * m);
       const int start = j * q + min(j, r), size = q + (j < r);
-      const int64_t kv = int_at(a.kv_len, a.kv_i64, b);
       const int4 e0 = make_int4(b, h, j, static_cast<int>(m));
-      const int4 e1 = make_int4(start * kTile, static_cast<int>(min(kv, static_cast<int64_t>(start + size) * kTile)), 0, 0);
+      const int4 e1 = make_int4(start * kTile, min(len, (start + size) * kTile), 0, 0);
+      // (never past the lists, whatever becomes of the lengths meanwhile)
+      const int64_t slot = static_cast<int64_t>(base) * H + i;
+      if (slot >= (dealt ? kPlanDealt : a.work_cap)) break;
       int4* const e = dealt ? s_item : work;
-      e[2 * (static_cast<int64_t>(base) * H + i)] = e0;
-      e[2 * (static_cast<int64_t>(base) * H + i) + 1] = e1;
+      e[2 * slot] = e0;
+      e[2 * slot + 1] = e1;
     }
     base += all;
     __syncthreads();
