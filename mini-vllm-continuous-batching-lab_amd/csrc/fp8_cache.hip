@@ -198,6 +198,13 @@ struct Fp8WriteArgs {
   int32_t write_groups;  // work groups of the cache write; those after it rotate rows
 };
 
+// n / d, n >= 0, d > 0: the 64-bit division (100 instructions) only where n needs
+// it (a prompt's append 37.0 -> 36.0 us; the gather waits for its stores anyway).
+__device__ __forceinline__ int64_t quotient(int64_t n, int d) {
+  if ((n >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+
 template <int DTYPE>
 __device__ __forceinline__ int64_t clamped_position(const Fp8WriteArgs& a, int64_t t) {
   const int64_t p = a.positions[t];
@@ -217,7 +224,7 @@ __device__ __forceinline__ void rotate_pair(const uint4 x1, const uint4 x2, cons
 // The query rows (and with k_out the key rows), rotated: a thread owns 8 pairs
 // (d, d + D/2) of two heads of a token, which share the tables' values. (9 k
 // tokens at 28 / 4 x 128, outputs not in a cache: 38.5 us with one head a thread,
-// 36.4 with two, 36.9 with four. Non-temporal stores take another 2 off, and
+// 36.8 with two, no better with four. Non-temporal stores take another 2 off, and
 // give it back in the attention that reads the rows next.)
 constexpr int kRotHeads = 2;
 
@@ -228,9 +235,9 @@ __device__ __forceinline__ void rotate_rows(const Fp8WriteArgs& a, int group, in
   const int sets = (heads + kRotHeads - 1) / kRotHeads;
   const int64_t total = static_cast<int64_t>(a.num_tokens) * sets * kPer;
   for (int64_t i = static_cast<int64_t>(group) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(groups) * 256) {
-    const int c = static_cast<int>(i % kPer);
+    const int c = static_cast<int>(i & (kPer - 1));
     const int64_t ts = i / kPer;
-    const int64_t t = ts / sets;
+    const int64_t t = quotient(ts, sets);
     const int h0 = static_cast<int>(ts - t * sets) * kRotHeads;
     const int64_t row = clamped_position<DTYPE>(a, t) * a.table_stride;
     const int o1 = c * 16, o2 = o1 + D;
@@ -296,7 +303,7 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
 // dependent loads (plan words; row, position and scale; cos and sin; codes
 // that shrink): 3.0 us for one row at 14 / 2 x 64 with the query's rotation,
 // 4.2 for 64 (3.25 and 4.45 with the plan's words in two rounds and the wave's
-// maximum through LDS). A prompt's is bound by its bytes: 36.4 us for 166 MB (9 k
+// maximum through LDS). A prompt's is bound by its bytes: 36.0 us for 166 MB (9 k
 // tokens at 28 / 4 x 128, rotation and returned key), 4.6 TB/s, nine tenths of a
 // large copy's rate; 30 where the outputs' memory is still in a cache.
 template <int DTYPE, int D, bool FIT>
@@ -319,8 +326,8 @@ __device__ __forceinline__ void write_units(const Fp8WriteArgs& a) {
     const bool live = u < bound;
     const int j = static_cast<int>(u & 1);  // 0: K, 1: V
     const int64_t ih = live ? u >> 1 : 0;
-    const int h = static_cast<int>(ih % a.num_kv_heads);
-    const int64_t item = ih / a.num_kv_heads;
+    const int64_t item = quotient(ih, a.num_kv_heads);
+    const int h = static_cast<int>(ih - item * a.num_kv_heads);
     // the plan's words in one round of loads, the number of items among them:
     // what lies behind the last item is read and not used
     const int32_t* tab = a.table + (item << a.bs_log2);
